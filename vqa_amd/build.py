@@ -12,7 +12,11 @@ OUT = os.path.join(HERE, 'libvqa_amd.so')
 SOURCES = ['schedule.cpp', 'tree.cpp', 'prof.cpp', 'feed.cpp', 'conv.hip', 'conv_f32.hip', 'wgrad.hip', 'gemm.hip', 'misc.hip', 'adam.hip', 'devsched.hip', 'head.hip']
 HEADERS = ['vqa_dev.h', 'plan.h', 'prof.h', os.path.join('..', '..', 'include', 'vqa_amd.h')]
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-FLAGS = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=gfx950', '-Wall', '-Wno-unused-function']
+# no packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): some of its forms have given wrong results now and
+# then on this hardware, and the compiler makes them from ordinary float code.  (The host pass does not know the feature and
+# says so: harmless.)
+FLAGS = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=gfx950', '-Wall', '-Wno-unused-function',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 def _stale(target, deps):
