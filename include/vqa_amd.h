@@ -32,6 +32,11 @@ extern "C" {
 
 #define VQA_HW 196     /* 14 x 14 pixels per feature map */
 
+/* element types of the row operators (vqa_sample, vqa_token_logp, vqa_dropout) */
+#define VQA_BF16 0
+#define VQA_F16 1
+#define VQA_F32 2
+
 int vqa_version(void);
 const char* vqa_last_error(void);
 
@@ -486,6 +491,40 @@ int vqa_head_backward(const float* dlogits, const void* act, int64_t ld_act, con
  * range adds nothing to either); workspace: 128 floats */
 int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlogits, float* workspace, int32_t N,
              int32_t A, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Log-probability and entropy of one chosen token per row of logits, and their gradient: the score of sampled
+ * programs (Seq2Seq.reinforce_backward, LSTM_Model.py:261-278; program_to_probs, LSTM_Model.py:186).
+ *   p = softmax(x / temperature);  logp[r] = log p[r][token[r]];  entropy[r] = -sum p log p
+ *   dx = (g (onehot(token) - p) - h p (log p + entropy)) / temperature
+ * Row r of the logits starts at element (r / inner) * ld_outer + (r % inner) * ld_inner of x (any element strides, rows
+ * themselves contiguous); dtype VQA_BF16 / VQA_F16 / VQA_F32, pointers aligned to an element.  A token outside [0, V) or
+ * equal to `ignore` gives logp = entropy = 0 and zeros in dx; a row of nothing but -inf gives logp = -inf, entropy = 0 and
+ * zeros in dx; NaN or +inf in a row gives NaN.  Sums are fp32 in a fixed order.
+ * ------------------------------------------------------------------------------------------ */
+/* floats of workspace vqa_token_logp needs (0: none, the pointer may be null); 16-byte aligned */
+int64_t vqa_token_logp_workspace(int64_t rows, int32_t V, int32_t dtype);
+/* logp fp32 [rows]; entropy fp32 [rows] or null; stats fp32 [rows][4], 16-byte aligned: what the backward call needs */
+int vqa_token_logp(const void* x, int64_t inner, int64_t ld_inner, int64_t ld_outer, const int64_t* tokens, float* logp,
+                   float* entropy, float* stats, float* workspace, int64_t rows, int32_t V, int32_t dtype, float temperature,
+                   int64_t ignore, void* stream);
+/* g, h fp32 [rows]: d(loss)/d(logp) and d(loss)/d(entropy), either may be null; h needs stats of a call with `entropy`.
+ * dx [rows][V] dense, of the logits' type, written whole */
+int vqa_token_logp_backward(const void* x, int64_t inner, int64_t ld_inner, int64_t ld_outer, const int64_t* tokens,
+                            const float* stats, const float* g, const float* h, void* dx, int64_t rows, int32_t V, int32_t dtype,
+                            float temperature, int64_t ignore, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Dropout with a mask that is a function of (seed, offset, element index) and never stored: the backward pass is the same
+ * call on the incoming gradient.  Element i takes 16 bits of Philox4x32-10 (key = seed, counter = offset + i / 8; element
+ * i % 8 = 2 w + b: half b, low first, of word w) and is dropped - set to +0, whatever it was - iff they are below
+ * `threshold` in [0, 65536]; the others are multiplied by 65536 / (65536 - threshold).  `state`: null, or device
+ * {seed, offset} read in place of the two arguments when the kernel runs (a replayed graph draws new masks when the caller
+ * advances it).  n contiguous elements of `dtype`; y may be x.  A call uses the counters offset .. offset + (n + 7) / 8 - 1.
+ * No counterpart in the reference's default configuration (classifier_dropout, Module_Model.py:107).
+ * ------------------------------------------------------------------------------------------ */
+int vqa_dropout(const void* x, void* y, int64_t n, int32_t dtype, int32_t threshold, uint64_t seed, uint64_t offset,
+                const int64_t* state, void* stream);
 
 /* dst slot <- (sum of listed source slots) * (mask slot > 0): scene-node gradient fan-in
  * (feats[i:i+1] is read by every scene node of sample i, Module_Model.py:214) */

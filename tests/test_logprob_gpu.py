@@ -1,0 +1,238 @@
+"""Log-probability and entropy of chosen tokens and their gradient (vqa_amd.loss.token_log_probs over vqa_token_logp /
+vqa_token_logp_backward) against the formulas in 64 bits.
+
+Tolerances, with eps = 2^-24 (half a step of fp32): the sum of exponentials takes at most V / 256 + 64 additions one after
+the other and 14 merges, each of relative error eps, and an exponent of size r is off by at most 4 r eps (a subtraction, the
+constant, a product, the exponential itself).  So lp, H and log p are off by eps (V / 256 + 80 + 4 (|lp| + log V + 1)), and a
+gradient by that times its terms, half a step of its type, and half of the type's smallest number."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -126}
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def dev():
+    return torch.device('cuda:0')
+
+
+def reference(x, tokens, temperature, g, h):
+    """lp, H, dx, and the size of dx's terms, in 64 bits; rows without a live token or a finite logit as documented."""
+    z = x.double() / temperature
+    V = z.size(-1)
+    live = (tokens >= 0) & (tokens < V)
+    empty = (z == -math.inf).all(-1)
+    at = tokens.clamp(0, V - 1)[..., None]
+    zs = torch.where(empty[..., None], 0.0, z)
+    zs = zs - zs.amax(-1, keepdim=True)          # (log V is lost next to a row of 3e38, in 64 bits too)
+    logp = zs - torch.logsumexp(zs, -1, keepdim=True)
+    p = logp.exp()
+    fin = torch.where(p > 0, logp, 0.0)
+    ent = -(p * fin).sum(-1, keepdim=True)
+    one = torch.zeros_like(p).scatter_(-1, at, 1.0)
+    g, h = g.double()[..., None], h.double()[..., None]
+    dx = (g * (one - p) - h * p * (fin + ent)) / temperature
+    size = (g.abs() * (one + p) + h.abs() * p * (fin.abs() + ent)) / temperature
+    off = (~live | empty)[..., None]
+    lp = torch.where(empty, -math.inf, logp.gather(-1, at)[..., 0])
+    return (torch.where(live, lp, 0.0), torch.where(live & ~empty, ent[..., 0], 0.0), torch.where(off, 0.0, dx),
+            torch.where(off, 0.0, size), torch.where(off, 0.0, fin))
+
+
+def check(x, tokens, temperature=1.0, ignore=None, entropy=True, seed=0):
+    from vqa_amd.loss import token_log_probs
+    gen = torch.Generator().manual_seed(seed + 1)
+    g, h = torch.randn(tokens.shape, generator=gen), torch.randn(tokens.shape, generator=gen)
+    if not entropy:
+        h = torch.zeros_like(h)
+    xd = x.detach().requires_grad_(True)
+    out = token_log_probs(xd, tokens.to(dev()), temperature, ignore, entropy)
+    lp, ent = out if entropy else (out, None)
+    grads = (g.to(dev()), h.to(dev())) if entropy else (g.to(dev()),)
+    (dx,) = torch.autograd.grad(out if entropy else (out,), xd, grads)
+    assert lp.dtype == torch.float32 and lp.shape == tokens.shape and dx.dtype == x.dtype and dx.shape == x.shape
+    tk = torch.where(tokens == ignore, -1, tokens) if ignore is not None else tokens
+    rlp, rent, rdx, size, logp = reference(x.cpu(), tk, temperature, g, h)
+    V = x.size(-1)
+    tol = EPS * (V / 256 + 80 + 4 * (rlp.abs().nan_to_num(0, 0, 0) + math.log(V) + 1))
+    lp = lp.double().cpu()
+    assert torch.equal(lp == -math.inf, rlp == -math.inf)
+    fin = rlp > -math.inf
+    assert ((lp - rlp).abs()[fin] <= tol[fin]).all(), ((lp - rlp).abs()[fin] / tol[fin]).max()
+    if entropy:
+        # H is a mean of |log p|, whose error is that of each of its terms
+        assert ((ent.double().cpu() - rent).abs() <= EPS * (V / 256 + 80 + 8 * (math.log(V) + 1)) * (rent + 1)).all()
+    rel = EPS * (V / 256 + 80 + 4 * (logp.abs() + math.log(V) + 1))
+    bound = size * 2 * rel + rdx.abs() * torch.finfo(x.dtype).eps / 2 + TINY[x.dtype]
+    bad = (dx.double().cpu() - rdx).abs() > bound
+    assert not bad.any(), (bad.sum(), (dx.double().cpu() - rdx).abs()[bad][:5], bound[bad][:5])
+
+
+def logits(shape, seed, dtype, scale=3.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(dev())
+
+
+def tokens_for(shape, V, seed):
+    return torch.randint(0, V, shape, generator=torch.Generator().manual_seed(seed))
+
+
+# one token, the program vocabulary, sizes around every change of the number of threads a row has, odd and large ones
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows,V', [(1, 1), (3, 2), (7, 44), (5, 127), (6, 129), (4, 257), (9, 512), (3, 1025), (2, 4096),
+                                    (5, 4097), (3, 8191), (2, 50001), (1, 131072), (1030, 4100)])
+def test_values_and_gradients(dtype, rows, V):
+    check(logits((rows, V), rows * V, dtype), tokens_for((rows,), V, V), entropy=True)
+
+
+@pytest.mark.parametrize('V', [44, 1000, 6001])
+@pytest.mark.parametrize('temperature', [0.3, 1.7])
+@pytest.mark.parametrize('entropy', [True, False])
+def test_temperature(V, temperature, entropy):
+    check(logits((11, V), V, torch.float32), tokens_for((11,), V, 3), temperature, entropy=entropy)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('V', [44, 300, 5000, 20011])
+def test_masks_and_padding(dtype, V):
+    """-inf and the type's lowest value as masks, rows that nothing is left of, padding and tokens out of range, a chosen
+    token that is masked, a row whose every other token is masked."""
+    x = logits((12, V), V + 1, dtype)
+    tk = tokens_for((12,), V, 5)
+    x[0, 1:] = -math.inf
+    tk[0] = 0
+    x[1, :] = -math.inf
+    x[2, ::2] = -math.inf
+    x[3, ::3] = torch.finfo(dtype).min
+    x[4, :] = torch.finfo(dtype).min
+    tk[5], tk[6], tk[7] = -1, V, V + 2 ** 33
+    x[8, tk[8]] = -math.inf
+    x[5, 0] = math.nan                        # behind the end of a program: never looked at
+    x[9, : V // 2] = -math.inf
+    tk[10] = 7
+    check(x, tk, ignore=7)
+
+
+def test_nan_and_inf_rows():
+    from vqa_amd.loss import token_log_probs
+    for V in (44, 9000):
+        x = logits((4, V), 1, torch.float32)
+        x[1, 5] = math.nan
+        x[2, 6] = math.inf
+        x.requires_grad_(True)
+        lp, ent = token_log_probs(x, torch.zeros(4, dtype=torch.int64, device=dev()), entropy=True)
+        (dx,) = torch.autograd.grad(lp.sum() + ent.sum(), x)
+        for t in (lp, ent, dx.sum(1)):
+            assert t.isnan().tolist() == [False, True, True, False]
+
+
+def test_layouts_that_are_read_in_place_and_others():
+    """A slice over time steps (two strides), a column range of a wider tensor (odd start), a transposed tensor, a
+    broadcast row, one row without leading dimensions."""
+    base = logits((3, 6, 101), 2, torch.bfloat16)
+    tk = tokens_for((3, 5), 101, 1)
+    check(base[:, :-1], tk)
+    check(base[:, 1:, 3:44], tokens_for((3, 5), 41, 1))
+    check(base.permute(1, 0, 2), tokens_for((6, 3), 101, 2))
+    check(base.permute(2, 1, 0), tokens_for((101, 6), 3, 2))
+    check(base[0, 0].expand(4, 101), tokens_for((4,), 101, 2))
+    check(logits((2, 3, 4, 33), 3, torch.float32)[:, :2, 1:], tokens_for((2, 2, 3), 33, 3))
+    check(logits((77,), 3, torch.float32), tokens_for((), 77, 3))
+    from vqa_amd import ops
+    assert ops.row_layout(base[:, :-1])[0].data_ptr() == base.data_ptr()
+
+
+def test_broadcast_gradient_adds_over_its_rows():
+    from vqa_amd.loss import token_log_probs
+    x = logits((1, 50), 4, torch.float32).requires_grad_(True)
+    tk = tokens_for((6,), 50, 4).to(dev())
+    (dx,) = torch.autograd.grad(token_log_probs(x.expand(6, 50), tk).sum(), x)
+    each = [torch.autograd.grad(token_log_probs(x, tk[i:i + 1]).sum(), x)[0] for i in range(6)]
+    assert torch.allclose(dx, torch.stack(each).sum(0), rtol=0, atol=6 * 6 * EPS * 2)     # six terms of at most 1
+
+
+def test_no_rows():
+    from vqa_amd.loss import token_log_probs
+    x = torch.zeros(0, 44, device=dev(), requires_grad=True)
+    lp = token_log_probs(x, torch.zeros(0, dtype=torch.int64, device=dev()))
+    (dx,) = torch.autograd.grad(lp.sum(), x)
+    assert lp.shape == (0,) and dx.shape == (0, 44)
+
+
+def test_gradient_against_differences():
+    """Central differences of the 64-bit formula: step 1e-5, so 1e-10 from curvature and 1e-11 / 1e-5 from rounding."""
+    from vqa_amd.loss import token_log_probs
+    V, T = 23, 0.8
+    x = logits((2, V), 6, torch.float32, 1.5).requires_grad_(True)
+    tk = torch.tensor([4, 20])
+    lp, ent = token_log_probs(x, tk.to(dev()), T, entropy=True)
+    (dx,) = torch.autograd.grad(lp.sum() * 0.7 + ent.sum() * 0.3, x)
+
+    def f(z):
+        logp = torch.log_softmax(z / T, -1)
+        return 0.7 * logp.gather(1, tk[:, None]).sum() - 0.3 * (logp.exp() * logp).sum()
+    z = x.detach().double().cpu()
+    for r in range(2):
+        for i in range(V):
+            a, b = z.clone(), z.clone()
+            a[r, i] += 1e-5
+            b[r, i] -= 1e-5
+            assert abs((f(a) - f(b)).item() / 2e-5 - dx[r, i].item()) <= 2e-6 + 200 * EPS
+
+
+def test_same_bits_twice_and_on_another_stream():
+    from vqa_amd.loss import token_log_probs
+    x = logits((3, 70001), 8, torch.bfloat16).requires_grad_(True)
+    tk = tokens_for((3,), 70001, 8).to(dev())
+
+    def once():
+        lp, ent = token_log_probs(x, tk, entropy=True)
+        return lp.detach(), ent.detach(), torch.autograd.grad(lp.sum() + ent.sum(), x)[0]
+    a = once()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = once()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_captured_graph_replays_forward_and_backward():
+    from vqa_amd.loss import token_log_probs
+    x = logits((5, 9001), 9, torch.float32)
+    tk = tokens_for((5,), 9001, 9).to(dev())
+
+    def once(leaf):
+        lp, ent = token_log_probs(leaf, tk, entropy=True)
+        return lp.detach(), ent.detach(), torch.autograd.grad((lp.sum(), ent.sum()), leaf)[0]
+    leaf = x.clone().requires_grad_(True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        once(leaf)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once(leaf)
+    for k in range(3):
+        with torch.no_grad():
+            leaf.copy_(x * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = once((x * (k + 1)).requires_grad_(True))
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+def test_a_change_between_forward_and_backward_is_refused():
+    from vqa_amd.loss import token_log_probs
+    x = logits((2, 44), 1, torch.float32).requires_grad_(True)
+    lp = token_log_probs(x, torch.zeros(2, dtype=torch.int64, device=dev()))
+    with torch.no_grad():
+        x.add_(1)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        lp.sum().backward()

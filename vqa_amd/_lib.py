@@ -75,6 +75,7 @@ SEC = {name: i for i, name in enumerate((
     'SCENE_DPROJ_TILES'))}
 
 CONV_BIAS, CONV_RELU = 1, 2
+BF16, F16, F32 = 0, 1, 2
 TREE_UNFUSED, TREE_F32, TREE_SKIP_LEVEL0 = 1, 2, 4
 PLAN_SKIP_SEPARATE, PLAN_SKIP_FUSED, PLAN_BALANCE, PLAN_DEFER_BACKWARD = 1, 2, 4, 8
 
@@ -128,6 +129,10 @@ SIGNATURES = {
     'vqa_head_backward_workspace': (i64, [i32, i32, i32]),
     'vqa_head_backward': (i32, [vp, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i32, vp]),
     'vqa_xent': (i32, [vp, vp, vp, vp, vp, i32, i32, vp]),
+    'vqa_token_logp_workspace': (i64, [i64, i32, i32]),
+    'vqa_token_logp': (i32, [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, i32, i32, C.c_float, i64, vp]),
+    'vqa_token_logp_backward': (i32, [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, i32, i32, C.c_float, i64, vp]),
+    'vqa_dropout': (i32, [vp, vp, i64, i32, i32, C.c_uint64, C.c_uint64, vp, vp]),
     'vqa_gather_rows': (i32, [vp, i64, i64, vp, i64, vp, i32]),
     'vqa_adam_tensors': (i32, [vp, vp, i32, C.c_float, C.c_float, C.c_float, C.c_float, vp]),
     'vqa_adam_fc1': (i32, [vp, vp, vp, vp, vp, i32, i32, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float,

@@ -9,8 +9,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libvqa_amd.so')
-SOURCES = ['schedule.cpp', 'tree.cpp', 'prof.cpp', 'feed.cpp', 'conv.hip', 'conv_f32.hip', 'wgrad.hip', 'gemm.hip', 'misc.hip', 'adam.hip', 'devsched.hip', 'head.hip']
-HEADERS = ['vqa_dev.h', 'plan.h', 'prof.h', os.path.join('..', '..', 'include', 'vqa_amd.h')]
+SOURCES = ['schedule.cpp', 'tree.cpp', 'prof.cpp', 'feed.cpp', 'conv.hip', 'conv_f32.hip', 'wgrad.hip', 'gemm.hip', 'misc.hip', 'adam.hip', 'devsched.hip', 'head.hip',
+           'dropout.hip', 'logprob.hip']
+HEADERS = ['vqa_dev.h', 'plan.h', 'prof.h', 'rows.h', os.path.join('..', '..', 'include', 'vqa_amd.h')]
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 # no packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): some of its forms have given wrong results now and
 # then on this hardware, and the compiler makes them from ordinary float code.  (The host pass does not know the feature and

@@ -1,0 +1,87 @@
+"""Dropout from a counter-based generator: the mask is a function of (seed, offset, element index), computed in the forward
+and again in the backward pass, and never stored.
+
+    y = vqa_amd.dropout.dropout(x, 0.1, seed, offset)          # the caller's own counter
+    drop = vqa_amd.dropout.Dropout(0.1, seed=7)                # or a module that counts; y = drop(x)
+
+Element i (row-major) is dropped with probability p, rounded to a multiple of 2^-16; the others are multiplied by
+1 / (1 - p) for that rounded p.  Dropped elements become 0 whatever they were.  A call uses the counters offset to
+offset + ceil(numel / 8) - 1: calls whose ranges do not meet have independent masks, the same range gives the same mask.
+bf16, fp16 or fp32 on the GPU; there is no CPU path.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def blocks(numel):
+    """Counters that a call on `numel` elements uses."""
+    return (numel + 7) // 8
+
+
+def threshold(p):
+    """p in units of 2^-16, as the kernel takes it."""
+    p = float(p)
+    if not 0 <= p <= 1:
+        raise ValueError('dropout probability must be in [0, 1]')
+    return int(p * 65536 + 0.5)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, thr, seed, offset, state):
+        xc = x.detach().contiguous()
+        y = torch.empty_like(xc)
+        ops.dropout(xc, y, thr, seed, offset, state)
+        ctx.args = thr, seed, offset
+        ctx.save_for_backward(state)          # (changed before backward, it would give another mask: autograd refuses that)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (state,) = ctx.saved_tensors
+        dyc = dy.contiguous()
+        dx = torch.empty_like(dyc)
+        ops.dropout(dyc, dx, *ctx.args, state)
+        return dx, None, None, None, None
+
+
+def dropout(x, p, seed, offset=0):
+    """x with a share p of its elements set to 0 and the others multiplied by 1 / (1 - p).  `seed`, `offset`: integers, taken
+    modulo 2^64.  Or `seed` is an int64 tensor {seed, offset} on x's device, read by the kernels when they run: a captured
+    graph that advances it draws a new mask on every replay (advance it after the backward pass, not between)."""
+    if x.dtype not in ops.ROW_DTYPES:
+        raise ValueError('x must be bf16, fp16 or fp32')
+    thr = threshold(p)
+    ops._need_cuda(x)
+    state = None
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.shape != (2,) or not seed.is_contiguous() or seed.device != x.device or offset != 0:
+            raise ValueError('a seed tensor must be int64 [2] (seed, offset) on the device of x, without another offset')
+        seed, state = 0, seed
+    return _Dropout.apply(x, thr, int(seed), int(offset), state)
+
+
+class Dropout(torch.nn.Module):
+    """Dropout with a counter of its own: every training call takes the next range of counters of `seed`."""
+
+    def __init__(self, p=0.5, seed=0):
+        super().__init__()
+        threshold(p)
+        self.p, self.seed, self.offset = float(p), int(seed), 0
+
+    def forward(self, x):
+        if not self.training or self.p == 0:
+            return x
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            # the counter would be a constant of the graph: the same mask on every replay
+            raise RuntimeError('vqa_amd.dropout.Dropout counts on the host: in a captured graph call '
+                               'vqa_amd.dropout.dropout with a {seed, offset} tensor')
+        y = dropout(x, self.p, self.seed, self.offset)
+        self.offset += blocks(x.numel())
+        return y
+
+    def extra_repr(self):
+        return 'p=%g, seed=%d' % (self.p, self.seed)

@@ -7,8 +7,15 @@ Train_model.py:185,312 takes seven: log-softmax, gather, mean, and their gradien
 Mean reduction over the batch, no class weights, no label smoothing, targets int64 in [0, num_answers):
 the reference's call.  The forward kernel also writes d(loss)/d(logits); backward multiplies it by the
 incoming gradient.  fp32 logits on the GPU only: there is no CPU path.
+
+Log-probability and entropy of sampled program tokens, differentiable: the score of a policy gradient
+(Seq2Seq.reinforce_backward, LSTM_Model.py:261-278), for any vocabulary, in bf16, fp16 or fp32.
+
+    lp, ent = vqa_amd.loss.token_log_probs(logits, programs, ignore_index=0, entropy=True)   # [N, T] each
+    (-(reward[:, None] * lp).sum() - 0.01 * ent.sum()).backward()
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -41,3 +48,54 @@ def cross_entropy(logits, target):
 class CrossEntropyLoss(torch.nn.Module):
     def forward(self, logits, target):
         return _Xent.apply(logits, target)
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, ignore, want_entropy):
+        ctx.set_materialize_grads(False)
+        V = logits.size(-1)
+        x, *layout = ops.row_layout(logits.detach())
+        tk = tokens.contiguous()
+        f32 = dict(dtype=torch.float32, device=x.device)
+        lp = torch.empty(tokens.shape, **f32)
+        ent = torch.empty(tokens.shape, **f32) if want_entropy else None
+        stats = torch.empty(layout[0], 4, **f32)
+        if layout[0]:
+            ops.token_logp(x, layout, tk, lp, ent, stats, V, temperature, ignore)
+        # (the caller's own tensor where it was read in place: autograd then notices a change before backward)
+        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, tk, stats)
+        ctx.args = layout, V, temperature, ignore
+        return (lp, ent) if want_entropy else lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, h=None):
+        x, tk, stats = ctx.saved_tensors
+        layout, V, temperature, ignore = ctx.args
+        if g is None and h is None:
+            return None, None, None, None, None
+        dx = torch.empty(tuple(tk.shape) + (V,), dtype=x.dtype, device=x.device)
+        if layout[0]:
+            g, h = (t.contiguous() if t is not None else None for t in (g, h))
+            ops.token_logp_backward(x, layout, tk, stats, g, h, dx, V, temperature, ignore)
+        return dx, None, None, None, None
+
+
+def token_log_probs(logits, tokens, temperature=1.0, ignore_index=None, entropy=False):
+    """log softmax(logits / temperature) at `tokens`, fp32 of the tokens' shape; with `entropy` a pair of that and the
+    entropy of each row's distribution.  Both are differentiable with respect to the logits (once).
+
+    logits [..., V]: bf16, fp16 or fp32 on the GPU, rows at up to two strides are read in place (a slice over time steps);
+    tokens [...]: int64.  A token equal to `ignore_index` or outside [0, V) (padding behind a program's end) gives 0 and no
+    gradient.  -inf masks a token out; a row with nothing else gives -inf, entropy 0 and no gradient."""
+    if logits.dtype not in ops.ROW_DTYPES or logits.dim() < 1 or logits.size(-1) < 1:
+        raise ValueError('logits must be [..., V] in bf16, fp16 or fp32')
+    if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1]:
+        raise ValueError('tokens must be int64 of shape %s' % (tuple(logits.shape[:-1]),))
+    temperature = float(temperature)
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError('temperature must be in [1e-6, 1e6]')
+    ops._same_device(logits, tokens)
+    ignore = -1 if ignore_index is None else int(ignore_index)
+    return _TokenLogProbs.apply(logits, tokens, temperature, ignore, bool(entropy))

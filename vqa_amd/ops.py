@@ -319,6 +319,77 @@ def xent(logits, target, loss, dlogits):
     _lib.check(_lib.load().vqa_xent(_ptr(logits), _ptr(target), _ptr(loss), _ptr(dlogits), _ptr(ws), n, a, _stream()))
 
 
+ROW_DTYPES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+
+
+def _same_device(t, *ts):
+    _need_cuda(t, *ts)
+    for o in ts:
+        if o is not None and o.device != t.device:
+            raise ValueError('tensors on different devices: %s and %s' % (t.device, o.device))
+
+
+def row_layout(x):
+    """(x, rows, inner, ld_inner, ld_outer) of logits [..., V]: row r starts at element
+    (r // inner) * ld_outer + (r % inner) * ld_inner.  A tensor whose leading dimensions are not two strides over contiguous
+    rows is copied first."""
+    if x.size(-1) > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    dims = []                                   # [size, stride], outermost first, neighbours merged where they run on
+    for n, st in zip(x.shape[:-1], x.stride()[:-1]):
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == st * n:
+            dims[-1] = [dims[-1][0] * n, st]
+        else:
+            dims.append([n, st])
+    if len(dims) > 2:
+        x = x.contiguous()
+        dims = [[x.numel() // x.size(-1), x.size(-1)]]
+    while len(dims) < 2:
+        dims.insert(0, [1, 0])
+    return x, dims[0][0] * dims[1][0], max(1, dims[1][0]), dims[1][1], dims[0][1]
+
+
+def token_logp(x, layout, tokens, logp, entropy, stats, V, temperature, ignore):
+    """logp, entropy (or None) fp32 [rows], stats fp32 [rows, 4] of int64 tokens [rows] under softmax(x / temperature);
+    layout: (rows, inner, ld_inner, ld_outer) of x"""
+    rows, inner, ld_inner, ld_outer = layout
+    _same_device(x, tokens, logp, entropy, stats)
+    assert tokens.dtype == torch.int64 and tokens.is_contiguous() and tokens.numel() == rows
+    assert logp.dtype == stats.dtype == torch.float32 and logp.numel() == rows and stats.numel() == 4 * rows
+    assert entropy is None or (entropy.dtype == torch.float32 and entropy.numel() == rows)
+    lib, dt = _lib.load(), ROW_DTYPES[x.dtype]
+    with torch.cuda.device(x.device):
+        need = lib.vqa_token_logp_workspace(rows, V, dt)
+        ws = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
+        _lib.check(lib.vqa_token_logp(_ptr(x), inner, ld_inner, ld_outer, _ptr(tokens), _ptr(logp), _ptr(entropy), _ptr(stats),
+                                      _ptr(ws), rows, V, dt, temperature, ignore, _stream()))
+
+
+def token_logp_backward(x, layout, tokens, stats, g, h, dx, V, temperature, ignore):
+    """dx [rows, V] dense, of x's type; g, h: fp32 [rows] or None"""
+    rows, inner, ld_inner, ld_outer = layout
+    _same_device(x, tokens, stats, g, h, dx)
+    for t in (g, h):
+        assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() == rows)
+    assert dx.dtype == x.dtype and dx.is_contiguous() and dx.numel() == rows * V
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().vqa_token_logp_backward(_ptr(x), inner, ld_inner, ld_outer, _ptr(tokens), _ptr(stats), _ptr(g),
+                                                       _ptr(h), _ptr(dx), rows, V, ROW_DTYPES[x.dtype], temperature, ignore,
+                                                       _stream()))
+
+
+def dropout(x, y, threshold, seed, offset, state=None):
+    """y = x with the elements dropped whose random bits are below threshold (vqa_dropout); y may be x"""
+    _same_device(x, y, state)
+    assert x.dtype == y.dtype and x.is_contiguous() and y.is_contiguous() and y.numel() >= x.numel()
+    assert state is None or (state.dtype == torch.int64 and state.is_contiguous() and state.numel() == 2)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().vqa_dropout(_ptr(x), _ptr(y), x.numel(), ROW_DTYPES[x.dtype], threshold, seed & 2 ** 64 - 1,
+                                           offset & 2 ** 64 - 1, _ptr(state), _stream()))
+
+
 def slot_sum_mask(arena, blob, off_offsets, off_src, off_dst, off_mask, n_dst, slot_elems):
     b = blob.data_ptr()
     _lib.check(_lib.load().vqa_slot_sum_mask(_ptr(arena), C.c_void_p(b + 4 * off_offsets),
