@@ -493,6 +493,38 @@ int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlo
              int32_t A, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * One token per row of logits, drawn with given uniform numbers: a step of the program sampler on the device
+ * (Seq2Seq.reinforce_sample, LSTM_Model.py:205-235, which copies every step's tokens to the host), its tokens written
+ * straight into a column of the [N][T] int64 program array that vqa_devsched_build reads.
+ *   Order: descending logit, equal logits by index.  Weights: w = exp((x - max) / temperature).
+ *   Kept: the first top_k tokens; of these those with w >= min_p; of these the tokens whose exclusive cumulative weight is
+ *   below top_p times their total.  Drawn: the first kept token whose inclusive cumulative weight exceeds u times the kept
+ *   weight.  logp: log of its weight over the kept weight.
+ * Weights are exp in 64 bits rounded to a multiple of 2^-s, s = min(51, 62 - ceil(log2 V)), their sums exact: the same
+ * answer on every run.  -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw
+ * gets token -1 and logp -inf.  temperature <= 0 or NaN: the first token of the order, logp 0.  top_k <= 0, top_p >= 1, min_p <= 0
+ * (or NaN): off; top_p <= 0 or NaN, min_p >= 1: the first token, and with min_p its equals.  u below 0 or NaN counts as 0,
+ * u >= 1 draws the last kept token.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+    const void* logits;         /* row r at element r * ld; aligned to an element */
+    const float* u;             /* [rows] */
+    const float* temperature;   /* [rows], or null: temperature_value; likewise the next three */
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    int64_t* token;             /* out: token[r * ld_token] */
+    float* logp;                /* out [rows], or null */
+    int64_t ld, ld_token, rows;
+    double temperature_value, top_p_value, min_p_value;
+    int32_t top_k_value, V;
+    int32_t dtype;              /* VQA_BF16, VQA_F16, VQA_F32 */
+    int32_t reserved;
+} vqa_sample_params;
+
+int vqa_sample(const vqa_sample_params* p, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Log-probability and entropy of one chosen token per row of logits, and their gradient: the score of sampled
  * programs (Seq2Seq.reinforce_backward, LSTM_Model.py:261-278; program_to_probs, LSTM_Model.py:186).
  *   p = softmax(x / temperature);  logp[r] = log p[r][token[r]];  entropy[r] = -sum p log p

@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'libvqa_amd.so')
 SOURCES = ['schedule.cpp', 'tree.cpp', 'prof.cpp', 'feed.cpp', 'conv.hip', 'conv_f32.hip', 'wgrad.hip', 'gemm.hip', 'misc.hip', 'adam.hip', 'devsched.hip', 'head.hip',
-           'dropout.hip', 'logprob.hip']
+           'dropout.hip', 'logprob.hip', 'sample.hip']
 HEADERS = ['vqa_dev.h', 'plan.h', 'prof.h', 'rows.h', os.path.join('..', '..', 'include', 'vqa_amd.h')]
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 # no packed fp32 arithmetic (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32): some of its forms have given wrong results now and

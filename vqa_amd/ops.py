@@ -329,6 +329,43 @@ def _same_device(t, *ts):
             raise ValueError('tensors on different devices: %s and %s' % (t.device, o.device))
 
 
+def _call_on(t, fn, *args):
+    """fn(*args, stream) with t's device as the current one and its current stream.  (The handle is asked for directly:
+    torch.cuda.current_stream() takes 28 us in autograd's threads.)"""
+    i = t.get_device()
+    if i == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _lib.check(rc)
+
+
+def _addr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def sample(x, ld, rows, V, u, token, ld_token, logp, temperature, top_k, top_p, min_p):
+    """vqa_sample: token[r * ld_token] (and logp) of row r at element r * ld of x; the last four: a number, or one per row
+    (fp32, int32 for top_k)"""
+    p = _lib.SampleParams()
+    p.temperature_value, p.top_k_value, p.top_p_value, p.min_p_value = 1.0, 0, 1.0, 0.0
+    for name, v in (('temperature', temperature), ('top_k', top_k), ('top_p', top_p), ('min_p', min_p)):
+        if isinstance(v, torch.Tensor):
+            assert v.dtype == (torch.int32 if name == 'top_k' else torch.float32) and v.is_contiguous() and v.numel() == rows
+            _same_device(x, v)
+            setattr(p, name, v.data_ptr())
+        else:
+            setattr(p, name + '_value', v)
+    _same_device(x, u, token, logp)
+    assert u.dtype == torch.float32 and u.is_contiguous() and u.numel() == rows and token.dtype == torch.int64
+    assert logp is None or (logp.dtype == torch.float32 and logp.is_contiguous() and logp.numel() == rows)
+    p.logits, p.u, p.token, p.logp = x.data_ptr(), u.data_ptr(), token.data_ptr(), _addr(logp)
+    p.ld, p.ld_token, p.rows, p.V, p.dtype = ld, ld_token, rows, V, ROW_DTYPES[x.dtype]
+    _call_on(x, _lib.load().vqa_sample, C.byref(p))
+
+
 def row_layout(x):
     """(x, rows, inner, ld_inner, ld_outer) of logits [..., V]: row r starts at element
     (r // inner) * ld_outer + (r % inner) * ld_inner.  A tensor whose leading dimensions are not two strides over contiguous
@@ -360,11 +397,10 @@ def token_logp(x, layout, tokens, logp, entropy, stats, V, temperature, ignore):
     assert logp.dtype == stats.dtype == torch.float32 and logp.numel() == rows and stats.numel() == 4 * rows
     assert entropy is None or (entropy.dtype == torch.float32 and entropy.numel() == rows)
     lib, dt = _lib.load(), ROW_DTYPES[x.dtype]
-    with torch.cuda.device(x.device):
-        need = lib.vqa_token_logp_workspace(rows, V, dt)
-        ws = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
-        _lib.check(lib.vqa_token_logp(_ptr(x), inner, ld_inner, ld_outer, _ptr(tokens), _ptr(logp), _ptr(entropy), _ptr(stats),
-                                      _ptr(ws), rows, V, dt, temperature, ignore, _stream()))
+    need = lib.vqa_token_logp_workspace(rows, V, dt)
+    ws = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
+    _call_on(x, lib.vqa_token_logp, _addr(x), inner, ld_inner, ld_outer, _addr(tokens), _addr(logp), _addr(entropy), _addr(stats),
+             _addr(ws), rows, V, dt, temperature, ignore)
 
 
 def token_logp_backward(x, layout, tokens, stats, g, h, dx, V, temperature, ignore):
@@ -374,10 +410,8 @@ def token_logp_backward(x, layout, tokens, stats, g, h, dx, V, temperature, igno
     for t in (g, h):
         assert t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.numel() == rows)
     assert dx.dtype == x.dtype and dx.is_contiguous() and dx.numel() == rows * V
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().vqa_token_logp_backward(_ptr(x), inner, ld_inner, ld_outer, _ptr(tokens), _ptr(stats), _ptr(g),
-                                                       _ptr(h), _ptr(dx), rows, V, ROW_DTYPES[x.dtype], temperature, ignore,
-                                                       _stream()))
+    _call_on(x, _lib.load().vqa_token_logp_backward, _addr(x), inner, ld_inner, ld_outer, _addr(tokens), _addr(stats), _addr(g),
+             _addr(h), _addr(dx), rows, V, ROW_DTYPES[x.dtype], temperature, ignore)
 
 
 def dropout(x, y, threshold, seed, offset, state=None):
@@ -385,9 +419,8 @@ def dropout(x, y, threshold, seed, offset, state=None):
     _same_device(x, y, state)
     assert x.dtype == y.dtype and x.is_contiguous() and y.is_contiguous() and y.numel() >= x.numel()
     assert state is None or (state.dtype == torch.int64 and state.is_contiguous() and state.numel() == 2)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().vqa_dropout(_ptr(x), _ptr(y), x.numel(), ROW_DTYPES[x.dtype], threshold, seed & 2 ** 64 - 1,
-                                           offset & 2 ** 64 - 1, _ptr(state), _stream()))
+    _call_on(x, _lib.load().vqa_dropout, _addr(x), _addr(y), x.numel(), ROW_DTYPES[x.dtype], threshold, seed & 2 ** 64 - 1,
+             offset & 2 ** 64 - 1, _addr(state))
 
 
 def slot_sum_mask(arena, blob, off_offsets, off_src, off_dst, off_mask, n_dst, slot_elems):
