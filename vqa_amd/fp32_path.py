@@ -62,6 +62,7 @@ class _Fp32Path:
         dev = x.device
         N, c, p_, cin, cpad = x.size(0), d['c'], d['p'], d['cin'], d['cin_pad']
         f32t = torch.float32
+        drop = self._start_dropout(N)
         plan = Plan(program.detach().cpu().numpy(), self.vocab, c, self.wgrad_chunk, _lib.PLAN_SKIP_FUSED)
         info = plan.info
         self.used_fns = torch.from_numpy(plan.used_fns()).to(program.device)
@@ -69,7 +70,7 @@ class _Fp32Path:
         if self.plan_ready_hook is not None:
             self.plan_ready_hook(self.last_token_counts, dev, need_grad)
         ws = self._pool.acquire()
-        st = _CallState(N=N, plan=plan, f32=True, x_dtype=x.dtype, ws=ws)
+        st = _CallState(N=N, plan=plan, f32=True, x_dtype=x.dtype, ws=ws, drop=drop)
         try:
             st['pk'] = pk = self._weights_f32(dev)
             blob_host = torch.from_numpy(plan.blob())
@@ -116,6 +117,7 @@ class _Fp32Path:
                 if last:
                     st['logits'] = out
                 else:
+                    self._drop_hidden(drop, li, out[:N * fo])
                     acts.append(out)
                     prev_dim = fo
             st['acts'] = acts
@@ -155,6 +157,8 @@ class _Fp32Path:
             # input gradient, times (input > 0): the input came out of a ReLU
             gin = ws.get('fc32_gin%d' % li, N * fi, torch.float32, dev)
             ops.gemm_f32(g, lin.weight.detach(), gin, N, fi, fo, lda=g_ld, ldb=fi, ldc=fi, b_kmajor=True, mask=acts[li])
+            if li > 0:
+                self._drop_hidden(st['drop'], li - 1, gin[:N * fi])
             g, g_ld = gin, fi
         dc1 = ws.get('dc1_32', N * HW * p_, torch.float32, dev)      # back to channels-last [N][196][P]
         ops.transpose_f32(g, dc1, N, p_, HW)

@@ -15,7 +15,7 @@ import numpy as np
 import torch
 import torch.nn as nn
 
-from . import _lib, ops, vocab as V
+from . import _lib, dropout, ops, vocab as V
 from .schedule import Plan
 from .feed import FeatureRows
 
@@ -215,6 +215,13 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
         self.backward_order = os.environ.get('VQA_BWD_ORDER', 'A')
         self.schedule_error = None
         self._arity_dev = None
+        # dropout on every hidden layer of the classifier (behind its ReLU) while the module is in training mode: the
+        # opt-in for the reference's classifier_dropout, under the default network's state-dict keys.  Masks come from
+        # vqa_amd.dropout: a function of dropout_seed (plus the data-parallel rank) and dropout_offset, which every
+        # such call advances; nothing is stored for backward
+        self.hidden_dropout = 0.0
+        self.dropout_seed = 0
+        self.dropout_offset = 0
         self.keep_state = False       # tests: keep the last call's buffers in self.last_state
         # list-of-dicts programs: False = the reference's behaviour (AttributeError); True = run them
         self.accept_program_lists = False
@@ -407,8 +414,9 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
         if self.precision != 'bf16':
             raise ValueError("precision must be 'bf16' or 'fp32'")
         T = program.size(1)
+        drop = self._start_dropout(N)
         ws = self._pool.acquire()
-        st = _CallState(N=N, ws=ws, x_dtype=x.dtype if isinstance(x, torch.Tensor) else torch.float32)
+        st = _CallState(N=N, ws=ws, drop=drop, x_dtype=x.dtype if isinstance(x, torch.Tensor) else torch.float32)
         try:
             cur = torch.cuda.current_stream(dev)
             if self._side is None or self._side.device != dev:
@@ -653,6 +661,7 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
                 if np128 != N:
                     a.view(np128, fo)[N:].zero_()
                 ops.bias_act(acc, lin.bias.detach(), a, N, fo, fo, fo, True, slabs=split, slab_stride=N * fo)
+                self._drop_hidden(drop, li, a[:N * fo])
                 acts.append(a)
                 prev_dim = fo
         st['acts'] = acts
@@ -670,6 +679,26 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
         if self.keep_state:
             self.last_state = st
         return st
+
+    def _start_dropout(self, N):
+        """(threshold, seed, offset of each hidden layer) of a call with hidden_dropout, None without."""
+        thr = dropout.threshold(self.hidden_dropout)
+        if not self.training or thr == 0:
+            return None
+        seed = int(self.dropout_seed)
+        if torch.distributed.is_available() and torch.distributed.is_initialized():
+            seed += torch.distributed.get_rank()
+        at = []
+        for fo in self._dims['fcs']:
+            at.append(self.dropout_offset)
+            self.dropout_offset += dropout.blocks(N * fo)
+        return thr, seed, at
+
+    def _drop_hidden(self, drop, layer, t):
+        """Dropout of hidden layer `layer` in place, on its activations or on the gradient into them."""
+        if drop is not None:
+            thr, seed, at = drop
+            ops.dropout(t, t, thr, seed, at[layer])
 
     def _head_fused(self, fcs, dims_in):
         """Whether the last linear layer runs as vqa_head_forward / vqa_head_backward."""
@@ -820,6 +849,11 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
                 gin.view(np128, fi)[N:].zero_()   # rows past N are the K padding of the next GEMM
             wk = ws.get('head_ws', ops.head_backward_workspace(N, fi, fo), torch.float32, dev)
             ops.head_backward(dl, acts[li], fi, pk['fc_w'][li], fi, gin, fi, gw, gb_in, gb, wk, N, fi, fo)
+            if st['drop'] is not None:
+                # what was dropped is 0, so the ReLU mask has taken it out of gin already: the rest is scaled
+                self._drop_hidden(st['drop'], li - 1, gin[:N * fi])
+                gb_in.zero_()
+                ops.col_sum(gin, gb_in, N, fi, fi)
             if self.grad_ready_hook is not None:
                 self.grad_ready_hook(name + '.weight', gw)
                 emitted.add(name + '.weight')
@@ -869,6 +903,7 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
                      out_bf16=True, mask=acts[li])
             g, g_ld = gin, fi
             if li > 0:
+                self._drop_hidden(st['drop'], li - 1, gin[:N * fi])
                 gb = torch.zeros(fi, **f32)
                 ops.col_sum(gin, gb, N, fi, fi)
                 grads['classifier.%d.bias' % self._fc_idx[li - 1]] = gb
