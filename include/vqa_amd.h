@@ -497,7 +497,7 @@ int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlo
  * (Seq2Seq.reinforce_sample, LSTM_Model.py:205-235, which copies every step's tokens to the host), its tokens written
  * straight into a column of the [N][T] int64 program array that vqa_devsched_build reads.
  *   Order: descending logit, equal logits by index.  Weights: w = exp((x - max) / temperature).
- *   Kept: the first top_k tokens; of these those with w >= min_p; of these the tokens whose exclusive cumulative weight is
+ *   Kept: the first top_k tokens; of these those with w >= min_p ((x - max) / temperature >= log min_p); of these the tokens whose exclusive cumulative weight is
  *   below top_p times their total.  Drawn: the first kept token whose inclusive cumulative weight exceeds u times the kept
  *   weight.  logp: log of its weight over the kept weight.
  * Weights are exp in 64 bits rounded to a multiple of 2^-s, s = min(51, 62 - ceil(log2 V)), their sums exact: the same

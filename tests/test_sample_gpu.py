@@ -30,7 +30,7 @@ def draw_row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     live = x[order] > -np.inf
     e = np.where(live, np.exp(z), 0.0)
     if min_p > 0:
-        live &= e >= min(min_p, 1.0)
+        live &= z >= math.log(min(min_p, 1.0))     # (as logarithms: exp rounds to 1 next to 0)
     n = int(live.sum())
     w = [int(v) for v in np.rint(e[:n] * 2.0 ** s)]
     if top_k > 0:
@@ -210,3 +210,38 @@ def test_another_stream_and_a_captured_graph():
             torch.cuda.synchronize()
             want = sample(x, u, top_p=0.8, return_log_probs=True)
             assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_lone_token_has_log_probability_zero():
+    from vqa_amd.sampling import sample
+    for V in (2, 44, 700, 9000):
+        x = torch.full((3, V), -math.inf, device=dev())
+        x[:, V - 1] = torch.tensor([0.3, -7.0, 1e30], device=dev())
+        tk, lp = sample(x, uniform(3, 1).to(dev()), temperature=0.7, top_p=0.9, return_log_probs=True)
+        assert tk.tolist() == [V - 1] * 3 and lp.tolist() == [0.0] * 3
+        x[:, 0] = x[:, V - 1]
+        tk, lp = sample(x, uniform(3, 1).to(dev()), top_k=1, return_log_probs=True)
+        assert tk.tolist() == [0] * 3 and lp.tolist() == [0.0] * 3
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('V', [1025, 5000, 30011])
+def test_lists_of_every_length(dtype, V):
+    """Around the capacity of the list of candidates (2048): top-k beyond it, many equal logits at the cut, a bin edge that
+    falls on 0 (symmetric rows), rows far from 0, tiny and huge spreads."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(10, V, generator=g) * 2
+    x[1] = torch.linspace(-10, 10, V)
+    x[2] = torch.randint(0, 3, (V,), generator=g).float()
+    x[3] = torch.randint(0, 40, (V,), generator=g) * 0.25
+    x[4] = 1000 + x[4]
+    x[5] = x[5] * 1e-4
+    x[6] = x[6] * 1e3
+    x[7, : V // 2] = 5.0
+    x[8] = torch.linspace(-1e-30, 1e-30, V)
+    x[9, 0] = -1e30
+    x = x.to(dtype).to(dev())
+    for params in (dict(), dict(top_k=2000), dict(top_k=2048), dict(top_k=2049, top_p=0.9), dict(top_p=0.7),
+                   dict(top_p=0.999, min_p=0.01), dict(min_p=1.0), dict(temperature=0.01, top_p=0.9), dict(temperature=100.0)):
+        for u in (0.0, 0.4, 0.93, 1 - 2.0 ** -24):
+            check(x, torch.full((10,), u), **params)

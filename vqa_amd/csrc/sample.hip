@@ -15,6 +15,10 @@
 // exp is evaluated in 64 bits: a draw compares sums of up to V weights with u times their sum, and with fp32 exponentials
 // (2^-22) one row in ten of a flat distribution over 10^5 tokens would get a neighbouring token.
 #include "rows.h"
+#include <float.h>
+
+// a bin or a comparison has to come out the same wherever it is computed: no sums fused into products but by fma()
+#pragma clang fp contract(off)
 
 struct SampleArgs {
     const void* x;
@@ -83,15 +87,17 @@ template <int DT> struct Weights {
     __device__ __forceinline__ uint64_t of(uint32_t k) const { return of_z(z(k)); }
 };
 
-struct RowParams { double t, top_p, min_p, u; int32_t k; bool greedy; };
+struct RowParams { double t, top_p, min_p, u; int32_t k; bool greedy, nucleus; };
 __device__ __forceinline__ RowParams row_params(const SampleArgs& P, int64_t row) {
     RowParams r;
     r.t = P.temperature ? (double)P.temperature[row] : P.temperature_s;
     r.top_p = P.top_p ? (double)P.top_p[row] : P.top_p_s;
     r.min_p = P.min_p ? (double)P.min_p[row] : P.min_p_s;
     r.k = P.top_k ? P.top_k[row] : P.top_k_s;
-    r.u = (double)P.u[row];
+    const double u = (double)P.u[row];
+    r.u = u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;
     r.greedy = !(r.t > 0.0);
+    r.nucleus = !(r.top_p >= 1.0);
     return r;
 }
 template <int DT> __device__ __forceinline__ Weights<DT> row_weights(const RowParams& r, uint32_t top, int shift) {
@@ -163,30 +169,30 @@ template <int DT> __global__ __launch_bounds__(256) void sample_wave_kernel(Samp
         };
         const bool kept = in && (r.k <= 0 || before < r.k);
         uint64_t total = sum(kept ? w : 0);
-        if (r.top_p < 1.0 || r.top_p != r.top_p) {
+        if (r.nucleus) {
             const uint64_t end = nucleus_end(r.top_p, total);
             total = sum(kept && mass < end ? w : 0);
         }
         const uint64_t t = drawn_place(r.u, total);
         const uint64_t m = __ballot(kept && mass <= t && t < mass + w);      // exactly one lane
         const int at = __ffsll((unsigned long long)m) - 1;
-        if (lane == at) sample_put<DT>(P, row, lane, z - log((double)total) + (double)P.shift * 0.6931471805599453);
+        if (lane == at) sample_put<DT>(P, row, lane, z - log(ldexp((double)total, -P.shift)));
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// Any V: a workgroup of BT threads a row.
-#define SAMPLE_BINS 2048
+// Radix search, for any V: a workgroup of BT threads a row.
+#define RADIX_BINS 2048
 
 struct Hist {
-    uint32_t cnt[SAMPLE_BINS];
-    unsigned long long mass[SAMPLE_BINS];
+    uint32_t cnt[RADIX_BINS];
+    unsigned long long mass[RADIX_BINS];
 };
 struct Place {                     // the key that holds a place of the order
     uint32_t key;
     uint64_t cnt_above, mass_above;      // tokens and weight in front of the first token with that key
 };
-struct SampleShared {
+struct RadixShared {
     Hist h1, h2;
     unsigned long long scan_c[16], scan_m[16];
     uint32_t red[16];
@@ -197,7 +203,7 @@ struct SampleShared {
 
 template <int BT> struct Row {
     // the bin of `h` (of `bins` ones) that holds place t, from the top, with c / m in front of the highest bin; all threads
-    static __device__ void find_bin(SampleShared& S, const Hist& h, int bins, bool by_mass, uint64_t t, uint64_t c, uint64_t m) {
+    static __device__ void find_bin(RadixShared& S, const Hist& h, int bins, bool by_mass, uint64_t t, uint64_t c, uint64_t m) {
         constexpr int WAVES = BT / 64;
         const int tid = threadIdx.x, per = (bins + BT - 1) / BT;
         uint64_t sc = 0, sm = 0;
@@ -278,10 +284,10 @@ template <int BT> struct Row {
         });
     }
     template <int DT>
-    static __device__ Place find(SampleShared& S, const typename Elem<DT>::type* x, int V, const Weights<DT>& W, bool by_mass, uint64_t t) {
+    static __device__ Place find(RadixShared& S, const typename Elem<DT>::type* x, int V, const Weights<DT>& W, bool by_mass, uint64_t t) {
         constexpr int B = Keys<DT>::BITS;
         Place p;
-        find_bin(S, S.h1, SAMPLE_BINS, by_mass, t, 0, 0);
+        find_bin(S, S.h1, RADIX_BINS, by_mass, t, 0, 0);
         uint32_t prefix = S.bin;
         int low = B - 11;                                    // bits that are still open
         while (low > 0) {
@@ -304,7 +310,7 @@ template <int BT> struct Row {
     // index of the (j + 1)-th token with this key: every wave counts a contiguous piece of the row, then the right one
     // looks closer
     template <int DT>
-    static __device__ int64_t locate(SampleShared& S, const typename Elem<DT>::type* x, int V, uint32_t key, uint64_t j) {
+    static __device__ int64_t locate(RadixShared& S, const typename Elem<DT>::type* x, int V, uint32_t key, uint64_t j) {
         constexpr int WAVES = BT / 64;
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const int piece = ((V + WAVES - 1) / WAVES + 63) / 64 * 64;
@@ -334,60 +340,457 @@ template <int BT> struct Row {
     }
 };
 
-template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_row_kernel(SampleArgs P) {
+// The whole answer for one row by radix search; `top` is the row's largest key (not masked), the row is not greedy.
+template <int DT, int BT>
+static __device__ __attribute__((noinline)) void radix_row(RadixShared& S, const SampleArgs& P, int64_t row, const RowParams& r, uint32_t top) {
     typedef typename Elem<DT>::type T;
     typedef Row<BT> R;
-    __shared__ SampleShared S;
     const int tid = threadIdx.x;
+    const T* x = (const T*)P.x + row * P.ld;
+    R::clear(S.h1, RADIX_BINS);
+    __syncthreads();
+    const Weights<DT> W = row_weights<DT>(r, top, P.shift);
+    R::template count<DT>(S.h1, x, P.V, W, Keys<DT>::BITS - 11, RADIX_BINS, 32, 0);
+    __syncthreads();
+    uint64_t n = 0, total = 0;
+    for (int b = tid & 63; b < RADIX_BINS; b += 64) {        // (every wave for itself)
+        n += S.h1.cnt[b];
+        total += S.h1.mass[b];
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        n += __shfl_xor((unsigned long long)n, d);
+        total += __shfl_xor((unsigned long long)total, d);
+    }
+    if (r.k > 0 && (uint64_t)r.k < n) {
+        const Place p = R::template find<DT>(S, x, P.V, W, false, (uint64_t)r.k - 1);
+        total = p.mass_above + ((uint64_t)r.k - p.cnt_above) * W.of(p.key);
+    }
+    if (r.nucleus) {
+        const uint64_t last = nucleus_end(r.top_p, total) - 1;
+        const Place p = R::template find<DT>(S, x, P.V, W, true, last);
+        const uint64_t w = W.of(p.key);
+        total = p.mass_above + ((last - p.mass_above) / w + 1) * w;
+    }
+    const uint64_t t = drawn_place(r.u, total);
+    const Place p = R::template find<DT>(S, x, P.V, W, true, t);
+    const int64_t at = R::template locate<DT>(S, x, P.V, p.key, (t - p.mass_above) / W.of(p.key));
+    if (tid == 0) sample_put<DT>(P, row, at, W.z(p.key) - log(ldexp((double)total, -P.shift)));
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// 64 < V <= LIST_ALL: every token goes on the list.  Above: three passes over the row -
+//   1. its maximum and minimum;
+//   2. a histogram over BINS equal steps of x below the maximum, down to where weights no longer count (e^-WINDOW).  With
+//      top-k, of tokens: the list is what is not below the k-th token's bin.  Without, of weight: a token of bin b weighs
+//      e^(-b d) e^(-f d) with |f| <= 1/2 and d <= 0.01, the second factor is a short polynomial (off by 2^-45 at most) and
+//      added as an integer; the bin's weight is that sum times e^(-b d), and a scan gives the weight in front of each bin;
+//   3. the list: the tokens of the bin that the nucleus ends in and of the bins that the draw can fall into.
+// The list (key and index of each token, LIST at most) is sorted in LDS, its weights are added up in order, and nucleus and
+// draw are looked up in it.  Rows whose list would be too long - many equal logits - go to the radix search.
+#define LIST_ALL 1024
+#define LIST 2048
+#define BINS 4096
+#define WINDOW 40.0
+
+typedef Keys<VQA_F32> FKeys;       // the list's keys: of the logits as fp32, whatever their type
+
+// Steps of x below the maximum: bin b holds the x with rint((max - x) scale) = b.
+struct Steps {
+    double max, scale;
+    __device__ __forceinline__ double at(float x) const { return (max - (double)x) * scale; }
+    static __device__ __forceinline__ uint32_t nearest(double a) {        // 0 <= a < 2^31
+        return (uint32_t)__double_as_longlong(a + 4503599627370496.0);
+    }
+    __device__ __forceinline__ uint32_t bin(float x) const { return nearest(at(x)); }
+};
+
+// One wave: the smallest float in [bottom, top] that `in` holds for; it holds for `top`, and for every float above one that
+// it holds for.  64 candidates a round.  (Stepping from a guess would not do: next to 0 there are millions of floats within
+// the rounding of max - x.)
+template <typename F> __device__ __forceinline__ float first_float(float bottom, float top, F in) {
+    uint32_t lo = FKeys::of(__float_as_uint(bottom)), hi = FKeys::of(__float_as_uint(top));
+    while (lo < hi) {
+        const uint32_t step = (hi - lo) / 64 + 1, lane = threadIdx.x & 63;
+        const uint32_t mine = lane <= (hi - lo) / step ? lo + lane * step : hi;
+        const uint64_t m = __ballot(in((float)FKeys::value(mine)));
+        if (m == 0) {
+            lo += 63 * step + 1;                             // (then lane 63 was below hi)
+        } else {
+            const uint32_t first = __ffsll((unsigned long long)m) - 1;
+            const uint32_t at = first <= (hi - lo) / step ? lo + first * step : hi;
+            lo = first ? lo + (first - 1) * step + 1 : at;
+            hi = at;
+        }
+    }
+    return (float)FKeys::value(hi);
+}
+
+template <int CAP> struct ListShared {
+    unsigned long long list[CAP];        // key << 32 | ~index: descending is the order
+    double w[CAP];
+    double part[16], total, behind;      // total: the kept weight; behind: the weight up to the nucleus's last bin
+    float max[16], min[16], edge[4], lo;
+    uint32_t n, last, pick, bin_end, bin_lo, bin_hi;
+};
+union BinShared {
+    unsigned long long mass[BINS];
+    uint32_t cnt[BINS];
+    double front[BINS];                  // the weight in front of each bin
+};
+
+// exclusive sums of v over the workgroup's threads, in thread order
+template <int BT> __device__ __forceinline__ double scan_threads(double* part, double v, double& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double inc = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(inc, d);
+        if (lane >= d) inc += o;
+    }
+    if (lane == 63) part[wave] = inc;
+    __syncthreads();
+    double base = 0.0, all = 0.0;
+#pragma unroll
+    for (int w = 0; w < BT / 64; w++) {
+        if (w < wave) base += part[w];
+        all += part[w];
+    }
+    __syncthreads();
+    total = all;
+    const double before = __shfl_up(inc, 1);
+    return lane ? base + before : base;
+}
+
+// descending bitonic sort of list[0, n); the list has room for the next power of two
+template <int BT> __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += BT) list[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            for (int p = threadIdx.x; p < size / 2; p += BT) {
+                const int a = 2 * p - (p & (j - 1)), b = a + j;
+                const unsigned long long va = list[a], vb = list[b];
+                if ((va < vb) == ((a & k) == 0)) {
+                    list[a] = vb;
+                    list[b] = va;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// Nucleus and draw in the sorted list of n tokens.  Without `front` the list holds all that is kept but for the nucleus;
+// with it, front[b] is the weight in front of bin b, `total` all weight, and the list holds the bins that matter.
+template <int DT, int BT, int CAP>
+__device__ __forceinline__ void finish_list(ListShared<CAP>& L, const SampleArgs& P, int64_t row, const RowParams& r,
+                                            const Weights<VQA_F32>& W, int n, double* front, const Steps& S, double total) {
+    const int tid = threadIdx.x, per = (n + BT - 1) / BT, i0 = min(n, tid * per), i1 = min(n, i0 + per);
+    double sum = 0.0, listed;
+    for (int i = i0; i < i1; i++) {
+        const double w = exp(W.z((uint32_t)(L.list[i] >> 32)));
+        L.w[i] = w;
+        sum += w;
+    }
+    if (tid == 0) L.last = L.pick = 0;
+    const double before = scan_threads<BT>(L.part, sum, listed);
+    auto bin_of = [&](int i) { return S.bin((float)FKeys::value((uint32_t)(L.list[i] >> 32))); };
+    if (front) {                                             // front[b] becomes what is in front of the bin beyond the list
+        double g = before;
+        for (int i = i0; i < i1; i++) {
+            const uint32_t b = bin_of(i);
+            if (i == 0 || bin_of(i - 1) != b) front[b] -= g;
+            g += L.w[i];
+        }
+        __syncthreads();
+    } else {
+        total = listed;
+    }
+    auto base = [&](int i) { return front ? front[bin_of(i)] : 0.0; };
+    uint32_t last = n - 1;
+    if (r.nucleus) {                                         // the last token in front of which less than `end` stands
+        const double end = r.top_p * total;
+        double g = before;
+        int mine = 0;
+        for (int i = i0; i < i1; i++) {
+            if (base(i) + g < end) mine = i;
+            g += L.w[i];
+        }
+        if (mine > 0) atomicMax(&L.last, (uint32_t)mine);
+        __syncthreads();
+        last = L.last;
+        if (i0 <= (int)last && (int)last < i1) {
+            double g = before;
+            for (int i = i0; i <= (int)last; i++) g += L.w[i];
+            L.total = base(last) + g;
+        }
+        __syncthreads();
+        total = L.total;
+    }
+    const double t = r.u * total;                            // drawn: the last kept token that does not start behind t
+    double g = before;
+    int mine = 0;
+    for (int i = i0; i < i1 && i <= (int)last; i++) {
+        if (base(i) + g <= t) mine = i;
+        g += L.w[i];
+    }
+    if (mine > 0) atomicMax(&L.pick, (uint32_t)mine);
+    __syncthreads();
+    if (tid == 0) {
+        const unsigned long long e = L.list[L.pick];
+        sample_put<DT>(P, row, (int64_t)(uint32_t)~(uint32_t)e, W.z((uint32_t)(e >> 32)) - log(total));
+    }
+}
+
+__device__ __forceinline__ unsigned long long list_entry(uint32_t key, int i) {
+    return ((unsigned long long)key << 32) | (uint32_t)~i;
+}
+template <int DT> __device__ __forceinline__ uint32_t float_key(const typename Elem<DT>::type* x, int64_t i) {
+    return FKeys::of(__float_as_uint(elem_get<DT>(x + i)));
+}
+
+template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_list_kernel(SampleArgs P) {
+    typedef typename Elem<DT>::type T;
+    constexpr int PER = LIST_ALL / BT;
+    __shared__ ListShared<LIST_ALL> L;
+    const int tid = threadIdx.x, V = P.V;
     for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
         const T* x = (const T*)P.x + row * P.ld;
-        uint32_t top = 0;
-        R::template each<DT>(x, P.V, [&](uint32_t key, int) { top = max(top, key); });
+        uint32_t key[PER], top = 0;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            key[k] = k * BT + tid < V ? float_key<DT>(x, k * BT + tid) : 0;
+            top = max(top, key[k]);
+        }
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        __syncthreads();                                     // (the previous row's use of S is over)
-        if ((tid & 63) == 0) S.red[tid >> 6] = top;
-        R::clear(S.h1, SAMPLE_BINS);
+        __syncthreads();                                     // (the previous row's use of L is over)
+        if ((tid & 63) == 0) L.max[tid >> 6] = __uint_as_float(top);
+        if (tid == 0) L.n = 0;
         __syncthreads();
-        for (int w = 0; w < BT / 64; w++) top = max(top, S.red[w]);
+        for (int w = 0; w < BT / 64; w++) top = max(top, __float_as_uint(L.max[w]));
+        if (top <= FKeys::MASKED) {
+            if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
+            continue;
+        }
+        RowParams r = row_params(P, row);
+        if (r.greedy) {                                      // the first token of the order
+            r.t = 1.0;
+            r.k = 1;
+        }
+        const Weights<VQA_F32> W = row_weights<VQA_F32>(r, top, P.shift);
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            const bool in = key[k] > FKeys::MASKED && W.z(key[k]) >= W.min_z;
+            L.list[k * BT + tid] = in ? list_entry(key[k], k * BT + tid) : 0;
+            mine += in;
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
+        if ((tid & 63) == 0) atomicAdd(&L.n, (uint32_t)mine);
+        sort_list<BT>(L.list, V);
+        int n = (int)L.n;
+        if (r.k > 0 && r.k < n) n = r.k;
+        finish_list<DT, BT, LIST_ALL>(L, P, row, r, W, n, nullptr, Steps(), 0.0);
+    }
+}
+
+template <int DT> __device__ __forceinline__ uint32_t own_key(float x) {      // a logit's key in its own type
+    if constexpr (DT == VQA_F32) return Keys<DT>::of(__float_as_uint(x));
+    else if constexpr (DT == VQA_BF16) return Keys<DT>::of(f2bf(x));
+    else return Keys<DT>::of(__builtin_bit_cast(uint16_t, (_Float16)x));
+}
+
+template <int DT, int BT> struct BinRow {
+    typedef typename Elem<DT>::type T;
+    // calls f(x, index) with every logit as a float
+    template <typename F> static __device__ __forceinline__ void each(const T* x, int V, F f) {
+        constexpr int N = Elem<DT>::N;
+        const int nv = V / N;
+        for (int v = threadIdx.x; v < nv; v += BT) {
+            const u32x4 r = vec_load<DT>(x + (int64_t)v * N);
+#pragma unroll
+            for (int k = 0; k < N; k++) f(vec_get<DT>(r, k), v * N + k);
+        }
+        for (int i = nv * N + threadIdx.x; i < V; i += BT) f(elem_get<DT>(x + i), i);
+    }
+    // front[b]: the sum of value(b') over b' < b; value reads mass / cnt, whose place front takes
+    template <typename F> static __device__ __forceinline__ double scan_bins(BinShared& B, double* part, double (&v)[BINS / BT], F value) {
+        constexpr int PER = BINS / BT;
+        double sum = 0.0, total;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            v[k] = value(threadIdx.x * PER + k);
+            sum += v[k];
+        }
+        double g = scan_threads<BT>(part, sum, total);
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            B.front[threadIdx.x * PER + k] = g;
+            g += v[k];
+        }
+        return total;
+    }
+    // the last bin with something in it that starts in front of (or, `upto`, at) t
+    static __device__ __forceinline__ void last_bin(const BinShared& B, const double (&v)[BINS / BT], uint32_t* out, double t, bool upto) {
+        constexpr int PER = BINS / BT;
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            const double g = B.front[threadIdx.x * PER + k];
+            if (v[k] > 0.0 && (upto ? g <= t : g < t)) mine = threadIdx.x * PER + k;
+        }
+        if (mine > 0) atomicMax(out, (uint32_t)mine);
+    }
+};
+
+template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_kernel(SampleArgs P) {
+    typedef typename Elem<DT>::type T;
+    typedef BinRow<DT, BT> R;
+    __shared__ union {
+        struct {
+            ListShared<LIST> L;
+            BinShared B;
+        } s;
+        RadixShared radix;
+    } shared;
+    ListShared<LIST>& L = shared.s.L;
+    BinShared& B = shared.s.B;
+    const int tid = threadIdx.x, wave = tid >> 6, V = P.V;
+    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
+        const T* x = (const T*)P.x + row * P.ld;
+        float max = -INFINITY, min = INFINITY;
+        R::each(x, V, [&](float f, int) {
+            max = fmaxf(max, f);                             // (a NaN is passed over)
+            min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
+        });
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            max = fmaxf(max, __shfl_xor(max, d));
+            min = fminf(min, __shfl_xor(min, d));
+        }
+        __syncthreads();                                     // (the previous row's use of LDS is over)
+        if ((tid & 63) == 0) {
+            L.max[wave] = max;
+            L.min[wave] = min;
+        }
+        if (tid == 0) L.n = L.bin_end = L.bin_lo = L.bin_hi = 0;
+        for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
         __syncthreads();
-        if (top <= Keys<DT>::MASKED) {
+#pragma unroll
+        for (int w = 0; w < BT / 64; w++) {
+            max = fmaxf(max, L.max[w]);
+            min = fminf(min, L.min[w]);
+        }
+        if (max == -INFINITY) {
             if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
             continue;
         }
         const RowParams r = row_params(P, row);
         if (r.greedy) {
-            const int64_t at = R::template locate<DT>(S, x, P.V, top, 0);
+            __syncthreads();                                 // (from here LDS is the other search's)
+            const int64_t at = Row<BT>::template locate<DT>(shared.radix, x, V, own_key<DT>(max), 0);
             if (tid == 0) sample_put<DT>(P, row, at, 0.0);
             continue;
         }
-        const Weights<DT> W = row_weights<DT>(r, top, P.shift);
-        R::template count<DT>(S.h1, x, P.V, W, Keys<DT>::BITS - 11, SAMPLE_BINS, 32, 0);
+        if (max == INFINITY || max == min) {
+            __syncthreads();
+            radix_row<DT, BT>(shared.radix, P, row, r, own_key<DT>(max));
+            continue;
+        }
+        const Weights<VQA_F32> W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
+        const double range = fmin((double)max - (double)min, WINDOW * r.t);
+        const Steps S = {(double)max, (BINS - 1) / range};
+        if (wave == 0) {
+            const float f = first_float(min, max, [&](float f) {
+                return (double)max - (double)f <= range && ((double)f - W.max) * W.inv_t >= W.min_z;
+            });
+            if (tid == 0) L.lo = f;
+        }
         __syncthreads();
-        uint64_t n = 0, total = 0;
-        for (int b = tid & 63; b < SAMPLE_BINS; b += 64) {   // (every wave for itself)
-            n += S.h1.cnt[b];
-            total += S.h1.mass[b];
+        const float lo = L.lo;
+        double v[BINS / BT], total = 0.0;
+        int k = r.k;
+        if (k > 0) {
+            R::each(x, V, [&](float f, int) {
+                if (f >= lo) atomicAdd(&B.cnt[S.bin(f)], 1u);
+            });
+            __syncthreads();
+            total = R::scan_bins(B, L.part, v, [&](int b) { return (double)B.cnt[b]; });
+            if (total <= (double)k) {                        // (the rest, if there is any, weighs nothing)
+                k = 0;
+                __syncthreads();
+                for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
+                __syncthreads();
+            }
         }
+        const bool by_count = k > 0;
+        if (by_count) {
+            R::last_bin(B, v, &L.bin_hi, (double)k, false);
+        } else {
+            const double d = W.inv_t / S.scale;              // a step of the bins in z
+            const double c1 = -d, c2 = d * d / 2, c3 = -d * d * d / 6, c4 = d * d * d * d / 24, one = 1.0 + W.magic;
+            const long long magic = __double_as_longlong(W.magic);
+            R::each(x, V, [&](float f, int) {
+                if (!(f >= lo)) return;
+                const double a = S.at(f), whole = a + 4503599627370496.0, e = a - (whole - 4503599627370496.0);
+                const double p = fma(e, fma(e, fma(e, fma(e, c4, c3), c2), c1), one);
+                atomicAdd(&B.mass[(uint32_t)__double_as_longlong(whole)], (unsigned long long)(__double_as_longlong(p) - magic));
+            });
+            __syncthreads();
+            total = R::scan_bins(B, L.part, v, [&](int b) {
+                const unsigned long long m = B.mass[b];
+                return m ? ldexp((double)m, -P.shift) * exp(-d * b) : 0.0;
+            });
+            if (r.nucleus) {
+                R::last_bin(B, v, &L.bin_end, r.top_p * total, false);
+                __syncthreads();
+                if (tid == (int)L.bin_end / (BINS / BT)) {
+                    double m = 0.0;
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            n += __shfl_xor((unsigned long long)n, d);
-            total += __shfl_xor((unsigned long long)total, d);
+                    for (int q = 0; q < BINS / BT; q++) m = q == (int)L.bin_end % (BINS / BT) ? v[q] : m;
+                    L.behind = B.front[L.bin_end] + m;
+                }
+                __syncthreads();
+                R::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
+                R::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
+            } else {
+                R::last_bin(B, v, &L.bin_lo, r.u * total, true);
+            }
         }
-        if (r.k > 0 && (uint64_t)r.k < n) {
-            const Place p = R::template find<DT>(S, x, P.V, W, false, (uint64_t)r.k - 1);
-            total = p.mass_above + ((uint64_t)r.k - p.cnt_above) * W.of(p.key);
+        __syncthreads();
+        // the tokens with edge 0 <= x < edge 1 or edge 2 <= x < edge 3 go on the list
+        if (wave < 4) {
+            const uint32_t end = L.bin_end;
+            const uint32_t first = by_count ? 0 : wave < 2 ? L.bin_lo : end;
+            const uint32_t last = by_count ? L.bin_hi : wave >= 2 ? end : r.nucleus ? ::min(L.bin_hi, end) : first;
+            float e = INFINITY;
+            if (!(wave & 1)) e = first_float(lo, max, [&](float f) { return S.bin(f) <= last; });
+            else if (first > 0) e = first_float(lo, max, [&](float f) { return S.bin(f) < first; });
+            if (wave >= 2 && (by_count || !r.nucleus)) e = INFINITY;
+            if ((tid & 63) == 0) L.edge[wave] = e;
         }
-        if (r.top_p < 1.0 || r.top_p != r.top_p) {
-            const uint64_t last = nucleus_end(r.top_p, total) - 1;
-            const Place p = R::template find<DT>(S, x, P.V, W, true, last);
-            const uint64_t w = W.of(p.key);
-            total = p.mass_above + ((last - p.mass_above) / w + 1) * w;
+        __syncthreads();
+        const float e0 = L.edge[0], e1 = L.edge[1], e2 = L.edge[2], e3 = L.edge[3];
+        R::each(x, V, [&](float f, int i) {
+            if ((f >= e0 && f < e1) || (f >= e2 && f < e3)) {
+                const uint32_t at = atomicAdd(&L.n, 1u);
+                if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), i);
+            }
+        });
+        __syncthreads();
+        int n = (int)L.n;
+        if (n > LIST) {
+            __syncthreads();
+            radix_row<DT, BT>(shared.radix, P, row, r, own_key<DT>(max));
+            continue;
         }
-        const uint64_t t = drawn_place(r.u, total);
-        const Place p = R::template find<DT>(S, x, P.V, W, true, t);
-        const int64_t at = R::template locate<DT>(S, x, P.V, p.key, (t - p.mass_above) / W.of(p.key));
-        if (tid == 0) sample_put<DT>(P, row, at, W.z(p.key) - log((double)total) + (double)P.shift * 0.6931471805599453);
+        sort_list<BT>(L.list, n);
+        if (by_count && k < n) n = k;
+        finish_list<DT, BT, LIST>(L, P, row, r, W, n, by_count ? nullptr : B.front, S, total);
     }
 }
 
@@ -426,11 +829,14 @@ extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     if (p->V <= 64) {                                                                                                     \
         const int64_t wg = (p->rows + 3) / 4;                                                                             \
         hipLaunchKernelGGL(sample_wave_kernel<DT>, dim3((unsigned)(wg < 65536 ? wg : 65536)), dim3(256), 0, s, P);        \
-    } else if (p->V <= 8192) {                                                                                            \
-        hipLaunchKernelGGL((sample_row_kernel<DT, 256>), dim3((unsigned)(p->rows < 65536 ? p->rows : 65536)), dim3(256), 0, s, P); \
+    } else if (p->V <= LIST_ALL) {                                                                                        \
+        hipLaunchKernelGGL((sample_list_kernel<DT, 256>), rows_grid, dim3(256), 0, s, P);                                  \
+    } else if (p->rows <= 256) {                                                                                          \
+        hipLaunchKernelGGL((sample_row_kernel<DT, 1024>), rows_grid, dim3(1024), 0, s, P);                                 \
     } else {                                                                                                              \
-        hipLaunchKernelGGL((sample_row_kernel<DT, 1024>), dim3((unsigned)(p->rows < 65536 ? p->rows : 65536)), dim3(1024), 0, s, P); \
+        hipLaunchKernelGGL((sample_row_kernel<DT, 512>), rows_grid, dim3(512), 0, s, P);                                   \
     }
+    const dim3 rows_grid((unsigned)(p->rows < 65536 ? p->rows : 65536));
     if (p->dtype == VQA_BF16) { SAMPLE_LAUNCH(VQA_BF16) }
     else if (p->dtype == VQA_F16) { SAMPLE_LAUNCH(VQA_F16) }
     else { SAMPLE_LAUNCH(VQA_F32) }
