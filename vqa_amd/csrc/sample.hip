@@ -16,6 +16,7 @@
 // (2^-22) one row in ten of a flat distribution over 10^5 tokens would get a neighbouring token.
 #include "rows.h"
 #include <float.h>
+#include <stdlib.h>
 
 // a bin or a comparison has to come out the same wherever it is computed: no sums fused into products but by fma()
 #pragma clang fp contract(off)
@@ -87,25 +88,33 @@ template <int DT> struct Weights {
     __device__ __forceinline__ uint64_t of(uint32_t k) const { return of_z(z(k)); }
 };
 
+// a value that all lanes of the wave agree on, held in scalar registers
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+__device__ __forceinline__ double uniform(double v) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+
 struct RowParams { double t, top_p, min_p, u; int32_t k; bool greedy, nucleus; };
 __device__ __forceinline__ RowParams row_params(const SampleArgs& P, int64_t row) {
     RowParams r;
-    r.t = P.temperature ? (double)P.temperature[row] : P.temperature_s;
-    r.top_p = P.top_p ? (double)P.top_p[row] : P.top_p_s;
-    r.min_p = P.min_p ? (double)P.min_p[row] : P.min_p_s;
+    r.t = uniform(P.temperature ? (double)P.temperature[row] : P.temperature_s);
+    r.top_p = uniform(P.top_p ? (double)P.top_p[row] : P.top_p_s);
+    r.min_p = uniform(P.min_p ? (double)P.min_p[row] : P.min_p_s);
     r.k = P.top_k ? P.top_k[row] : P.top_k_s;
     const double u = (double)P.u[row];
-    r.u = u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0;
+    r.u = uniform(u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0);
     r.greedy = !(r.t > 0.0);
     r.nucleus = !(r.top_p >= 1.0);
     return r;
 }
 template <int DT> __device__ __forceinline__ Weights<DT> row_weights(const RowParams& r, uint32_t top, int shift) {
     Weights<DT> w;
-    w.top = top;
-    w.max = Keys<DT>::value(top);
-    w.inv_t = 1.0 / r.t;
-    w.min_z = r.min_p > 0.0 ? log(r.min_p < 1.0 ? r.min_p : 1.0) : -INFINITY;
+    w.top = __builtin_amdgcn_readfirstlane(top);
+    w.max = uniform(Keys<DT>::value(top));
+    w.inv_t = uniform(1.0 / r.t);
+    w.min_z = r.min_p > 0.0 ? uniform(log(r.min_p < 1.0 ? r.min_p : 1.0)) : -INFINITY;
     w.magic = __longlong_as_double((long long)(1023 + 52 - shift) << 52);
     return w;
 }
@@ -340,15 +349,25 @@ template <int BT> struct Row {
     }
 };
 
-// The whole answer for one row by radix search; `top` is the row's largest key (not masked), the row is not greedy.
-template <int DT, int BT>
-static __device__ __attribute__((noinline)) void radix_row(RadixShared& S, const SampleArgs& P, int64_t row, const RowParams& r, uint32_t top) {
+// The rows that sample_row_kernel left: those whose token is LATER.
+#define LATER INT64_MIN
+template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_radix_kernel(SampleArgs P) {
     typedef typename Elem<DT>::type T;
     typedef Row<BT> R;
+    __shared__ RadixShared S;
     const int tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
+    if (P.token[row * P.ld_token] != LATER) continue;        // (the same for all threads: it is written behind a barrier)
     const T* x = (const T*)P.x + row * P.ld;
+    const RowParams r = row_params(P, row);
+    uint32_t top = 0;
+    R::template each<DT>(x, P.V, [&](uint32_t key, int) { top = max(top, key); });
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    if ((tid & 63) == 0) S.red[tid >> 6] = top;
     R::clear(S.h1, RADIX_BINS);
     __syncthreads();
+    for (int w = 0; w < BT / 64; w++) top = max(top, S.red[w]);
     const Weights<DT> W = row_weights<DT>(r, top, P.shift);
     R::template count<DT>(S.h1, x, P.V, W, Keys<DT>::BITS - 11, RADIX_BINS, 32, 0);
     __syncthreads();
@@ -376,6 +395,7 @@ static __device__ __attribute__((noinline)) void radix_row(RadixShared& S, const
     const Place p = R::template find<DT>(S, x, P.V, W, true, t);
     const int64_t at = R::template locate<DT>(S, x, P.V, p.key, (t - p.mass_above) / W.of(p.key));
     if (tid == 0) sample_put<DT>(P, row, at, W.z(p.key) - log(ldexp((double)total, -P.shift)));
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
@@ -428,7 +448,10 @@ template <typename F> __device__ __forceinline__ float first_float(float bottom,
 
 template <int CAP> struct ListShared {
     unsigned long long list[CAP];        // key << 32 | ~index: descending is the order
-    double w[CAP];
+    union {
+        double w[CAP];
+        unsigned long long other[CAP];
+    };
     double part[16], total, behind;      // total: the kept weight; behind: the weight up to the nucleus's last bin
     float max[16], min[16], edge[4], lo;
     uint32_t n, last, pick, bin_end, bin_lo, bin_hi;
@@ -462,15 +485,37 @@ template <int BT> __device__ __forceinline__ double scan_threads(double* part, d
     return lane ? base + before : base;
 }
 
-// descending bitonic sort of list[0, n); the list has room for the next power of two
-template <int BT> __device__ __forceinline__ void sort_list(unsigned long long* list, int n) {
+// *out = max(*out, v) where v, or 0, grows with the thread: the wave's last thread that has one asks for it
+__device__ __forceinline__ void raise(uint32_t* out, int v) {
+    const uint64_t m = __ballot(v > 0);
+    if (m && (threadIdx.x & 63) == 63 - __clzll((unsigned long long)m)) atomicMax(out, (uint32_t)v);
+}
+
+// Sorts list[0, n), descending; the answer is in `list` or, true, in `other`; both have room for the next power of two.
+// Short lists by counting what is larger than each entry, n * n / BT comparisons a thread without a barrier (n = 256, 1024
+// threads: 1 us); longer ones by a bitonic network, whose barriers cost 0.15 us each (n = 256: 36 of them).
+template <int BT> __device__ __forceinline__ bool sort_list(unsigned long long* list, unsigned long long* other, int n) {
+    const int tid = threadIdx.x;
+    if (n <= BT / 2) {
+        int parts = 2;                                       // threads an entry
+        while (parts < 64 && parts * 2 * n <= BT) parts *= 2;
+        const int i = tid / parts;
+        const unsigned long long mine = i < n ? list[i] : 0;
+        int rank = 0;
+        if (i < n)
+            for (int j = tid % parts; j < n; j += parts) rank += list[j] > mine;
+        for (int d = 1; d < parts; d <<= 1) rank += __shfl_xor(rank, d);
+        if (i < n && tid % parts == 0) other[rank] = mine;   // (entries differ: so do ranks)
+        __syncthreads();
+        return true;
+    }
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += BT) list[i] = 0;
+    for (int i = n + tid; i < size; i += BT) list[i] = 0;
     __syncthreads();
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int p = threadIdx.x; p < size / 2; p += BT) {
+            for (int p = tid; p < size / 2; p += BT) {
                 const int a = 2 * p - (p & (j - 1)), b = a + j;
                 const unsigned long long va = list[a], vb = list[b];
                 if ((va < vb) == ((a & k) == 0)) {
@@ -480,29 +525,33 @@ template <int BT> __device__ __forceinline__ void sort_list(unsigned long long* 
             }
             __syncthreads();
         }
+    return false;
 }
 
 // Nucleus and draw in the sorted list of n tokens.  Without `front` the list holds all that is kept but for the nucleus;
 // with it, front[b] is the weight in front of bin b, `total` all weight, and the list holds the bins that matter.
 template <int DT, int BT, int CAP>
-__device__ __forceinline__ void finish_list(ListShared<CAP>& L, const SampleArgs& P, int64_t row, const RowParams& r,
-                                            const Weights<VQA_F32>& W, int n, double* front, const Steps& S, double total) {
+__device__ __forceinline__ void finish_list(ListShared<CAP>& L, bool swapped, const SampleArgs& P, int64_t row,
+                                            const RowParams& r, const Weights<VQA_F32>& W, int n, double* front, const Steps& S,
+                                            double total) {
+    const unsigned long long* list = swapped ? L.other : L.list;         // (sorted; the weights take the other place)
+    double* weight = swapped ? (double*)L.list : L.w;
     const int tid = threadIdx.x, per = (n + BT - 1) / BT, i0 = min(n, tid * per), i1 = min(n, i0 + per);
     double sum = 0.0, listed;
     for (int i = i0; i < i1; i++) {
-        const double w = exp(W.z((uint32_t)(L.list[i] >> 32)));
-        L.w[i] = w;
+        const double w = exp(W.z((uint32_t)(list[i] >> 32)));
+        weight[i] = w;
         sum += w;
     }
     if (tid == 0) L.last = L.pick = 0;
     const double before = scan_threads<BT>(L.part, sum, listed);
-    auto bin_of = [&](int i) { return S.bin((float)FKeys::value((uint32_t)(L.list[i] >> 32))); };
+    auto bin_of = [&](int i) { return S.bin((float)FKeys::value((uint32_t)(list[i] >> 32))); };
     if (front) {                                             // front[b] becomes what is in front of the bin beyond the list
         double g = before;
         for (int i = i0; i < i1; i++) {
             const uint32_t b = bin_of(i);
             if (i == 0 || bin_of(i - 1) != b) front[b] -= g;
-            g += L.w[i];
+            g += weight[i];
         }
         __syncthreads();
     } else {
@@ -516,14 +565,14 @@ __device__ __forceinline__ void finish_list(ListShared<CAP>& L, const SampleArgs
         int mine = 0;
         for (int i = i0; i < i1; i++) {
             if (base(i) + g < end) mine = i;
-            g += L.w[i];
+            g += weight[i];
         }
-        if (mine > 0) atomicMax(&L.last, (uint32_t)mine);
+        raise(&L.last, mine);
         __syncthreads();
         last = L.last;
         if (i0 <= (int)last && (int)last < i1) {
             double g = before;
-            for (int i = i0; i <= (int)last; i++) g += L.w[i];
+            for (int i = i0; i <= (int)last; i++) g += weight[i];
             L.total = base(last) + g;
         }
         __syncthreads();
@@ -534,12 +583,12 @@ __device__ __forceinline__ void finish_list(ListShared<CAP>& L, const SampleArgs
     int mine = 0;
     for (int i = i0; i < i1 && i <= (int)last; i++) {
         if (base(i) + g <= t) mine = i;
-        g += L.w[i];
+        g += weight[i];
     }
-    if (mine > 0) atomicMax(&L.pick, (uint32_t)mine);
+    raise(&L.pick, mine);
     __syncthreads();
     if (tid == 0) {
-        const unsigned long long e = L.list[L.pick];
+        const unsigned long long e = list[L.pick];
         sample_put<DT>(P, row, (int64_t)(uint32_t)~(uint32_t)e, W.z((uint32_t)(e >> 32)) - log(total));
     }
 }
@@ -551,81 +600,98 @@ template <int DT> __device__ __forceinline__ uint32_t float_key(const typename E
     return FKeys::of(__float_as_uint(elem_get<DT>(x + i)));
 }
 
+// One row a workgroup, without a loop over rows: the compiler would keep the constants of exp and log in registers around it.
+#define GRID_X (1 << 20)
+__device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_list_kernel(SampleArgs P) {
     typedef typename Elem<DT>::type T;
     constexpr int PER = LIST_ALL / BT;
     __shared__ ListShared<LIST_ALL> L;
     const int tid = threadIdx.x, V = P.V;
-    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
-        const T* x = (const T*)P.x + row * P.ld;
-        uint32_t key[PER], top = 0;
+    const int64_t row = grid_row();
+    if (row >= P.rows) return;
+    const T* x = (const T*)P.x + row * P.ld;
+    uint32_t key[PER], top = 0;
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            key[k] = k * BT + tid < V ? float_key<DT>(x, k * BT + tid) : 0;
-            top = max(top, key[k]);
-        }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-        __syncthreads();                                     // (the previous row's use of L is over)
-        if ((tid & 63) == 0) L.max[tid >> 6] = __uint_as_float(top);
-        if (tid == 0) L.n = 0;
-        __syncthreads();
-        for (int w = 0; w < BT / 64; w++) top = max(top, __float_as_uint(L.max[w]));
-        if (top <= FKeys::MASKED) {
-            if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
-            continue;
-        }
-        RowParams r = row_params(P, row);
-        if (r.greedy) {                                      // the first token of the order
-            r.t = 1.0;
-            r.k = 1;
-        }
-        const Weights<VQA_F32> W = row_weights<VQA_F32>(r, top, P.shift);
-        int mine = 0;
-#pragma unroll
-        for (int k = 0; k < PER; k++) {
-            const bool in = key[k] > FKeys::MASKED && W.z(key[k]) >= W.min_z;
-            L.list[k * BT + tid] = in ? list_entry(key[k], k * BT + tid) : 0;
-            mine += in;
-        }
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
-        if ((tid & 63) == 0) atomicAdd(&L.n, (uint32_t)mine);
-        sort_list<BT>(L.list, V);
-        int n = (int)L.n;
-        if (r.k > 0 && r.k < n) n = r.k;
-        finish_list<DT, BT, LIST_ALL>(L, P, row, r, W, n, nullptr, Steps(), 0.0);
+    for (int k = 0; k < PER; k++) {
+        key[k] = k * BT + tid < V ? float_key<DT>(x, k * BT + tid) : 0;
+        top = max(top, key[k]);
     }
-}
-
-template <int DT> __device__ __forceinline__ uint32_t own_key(float x) {      // a logit's key in its own type
-    if constexpr (DT == VQA_F32) return Keys<DT>::of(__float_as_uint(x));
-    else if constexpr (DT == VQA_BF16) return Keys<DT>::of(f2bf(x));
-    else return Keys<DT>::of(__builtin_bit_cast(uint16_t, (_Float16)x));
-}
-
-template <int DT, int BT> struct BinRow {
-    typedef typename Elem<DT>::type T;
-    // calls f(x, index) with every logit as a float
-    template <typename F> static __device__ __forceinline__ void each(const T* x, int V, F f) {
-        constexpr int N = Elem<DT>::N;
-        const int nv = V / N;
-        for (int v = threadIdx.x; v < nv; v += BT) {
-            const u32x4 r = vec_load<DT>(x + (int64_t)v * N);
 #pragma unroll
-            for (int k = 0; k < N; k++) f(vec_get<DT>(r, k), v * N + k);
+    for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    if ((tid & 63) == 0) L.max[tid >> 6] = __uint_as_float(top);
+    if (tid == 0) L.n = 0;
+    __syncthreads();
+    for (int w = 0; w < BT / 64; w++) top = max(top, __float_as_uint(L.max[w]));
+    if (top <= FKeys::MASKED) {
+        if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
+        return;
+    }
+    RowParams r = row_params(P, row);
+    if (r.greedy) {                                      // the first token of the order
+        r.t = 1.0;
+        r.k = 1;
+    }
+    const Weights<VQA_F32> W = row_weights<VQA_F32>(r, top, P.shift);
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        const bool in = key[k] > FKeys::MASKED && W.z(key[k]) >= W.min_z;
+        L.list[k * BT + tid] = in ? list_entry(key[k], k * BT + tid) : 0;
+        mine += in;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
+    if ((tid & 63) == 0) atomicAdd(&L.n, (uint32_t)mine);
+    const bool swapped = sort_list<BT>(L.list, L.other, V);
+    int n = (int)L.n;
+    if (r.k > 0 && r.k < n) n = r.k;
+    finish_list<DT, BT, LIST_ALL>(L, swapped, P, row, r, W, n, nullptr, Steps(), 0.0);
+}
+
+// Passes over a row.  (Kept short: a pass runs once per row, and instructions that come from memory cost as much as the
+// row.  With the row held in registers and its passes unrolled, 75 KB of code, a row of 50001 took 12 us in the last pass
+// alone, 6 with these loops.)
+template <int DT, int BT> struct RowPass {
+    typedef typename Elem<DT>::type T;
+    static constexpr int N = Elem<DT>::N;
+    const T* x;
+    int V, nv;
+    __device__ __forceinline__ RowPass(const T* x_, int V_) : x(x_), V(V_), nv(V_ / N) {}
+    // calls f(x, index) with every logit as a float; U pieces of 16 bytes on their way at a time
+    template <int U, typename F> __device__ __forceinline__ void each(F f) const {
+        int v = threadIdx.x;
+#pragma unroll 1
+        for (; v + (U - 1) * BT < nv; v += U * BT) {
+            u32x4 r[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) r[k] = vec_load<DT>(x + (int64_t)(v + k * BT) * N);
+#pragma unroll
+            for (int k = 0; k < U; k++)
+#pragma unroll
+                for (int q = 0; q < N; q++) f(vec_get<DT>(r[k], q), (v + k * BT) * N + q);
         }
+        if (U > 1) {
+#pragma unroll 1
+            for (; v < nv; v += BT) {
+                const u32x4 r = vec_load<DT>(x + (int64_t)v * N);
+#pragma unroll
+                for (int q = 0; q < N; q++) f(vec_get<DT>(r, q), v * N + q);
+            }
+        }
+#pragma unroll 1
         for (int i = nv * N + threadIdx.x; i < V; i += BT) f(elem_get<DT>(x + i), i);
     }
-    // front[b]: the sum of value(b') over b' < b; value reads mass / cnt, whose place front takes
-    template <typename F> static __device__ __forceinline__ double scan_bins(BinShared& B, double* part, double (&v)[BINS / BT], F value) {
-        constexpr int PER = BINS / BT;
+};
+
+template <int BT> struct BinScan {
+    static constexpr int PER = BINS / BT;
+    // front[b]: the sum of v over the bins before b; v: the thread's bins, read from where front goes
+    static __device__ __forceinline__ double scan(BinShared& B, double* part, const double (&v)[PER]) {
         double sum = 0.0, total;
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            v[k] = value(threadIdx.x * PER + k);
-            sum += v[k];
-        }
+        for (int k = 0; k < PER; k++) sum += v[k];
         double g = scan_threads<BT>(part, sum, total);
 #pragma unroll
         for (int k = 0; k < PER; k++) {
@@ -635,75 +701,74 @@ template <int DT, int BT> struct BinRow {
         return total;
     }
     // the last bin with something in it that starts in front of (or, `upto`, at) t
-    static __device__ __forceinline__ void last_bin(const BinShared& B, const double (&v)[BINS / BT], uint32_t* out, double t, bool upto) {
-        constexpr int PER = BINS / BT;
+    static __device__ __forceinline__ void last_bin(const BinShared& B, const double (&v)[PER], uint32_t* out, double t, bool upto) {
         int mine = 0;
 #pragma unroll
         for (int k = 0; k < PER; k++) {
             const double g = B.front[threadIdx.x * PER + k];
             if (v[k] > 0.0 && (upto ? g <= t : g < t)) mine = threadIdx.x * PER + k;
         }
-        if (mine > 0) atomicMax(out, (uint32_t)mine);
+        raise(out, mine);
     }
 };
 
 template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_kernel(SampleArgs P) {
     typedef typename Elem<DT>::type T;
-    typedef BinRow<DT, BT> R;
-    __shared__ union {
-        struct {
-            ListShared<LIST> L;
-            BinShared B;
-        } s;
-        RadixShared radix;
-    } shared;
-    ListShared<LIST>& L = shared.s.L;
-    BinShared& B = shared.s.B;
-    const int tid = threadIdx.x, wave = tid >> 6, V = P.V;
-    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
-        const T* x = (const T*)P.x + row * P.ld;
-        float max = -INFINITY, min = INFINITY;
-        R::each(x, V, [&](float f, int) {
-            max = fmaxf(max, f);                             // (a NaN is passed over)
-            min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
-        });
+    constexpr int PER = BINS / BT;
+    __shared__ ListShared<LIST> L;
+    __shared__ BinShared B;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int64_t row = grid_row();
+    if (row >= P.rows) return;
+    const RowPass<DT, BT> H((const T*)P.x + row * P.ld, P.V);
+    const RowParams r = row_params(P, row);
+    for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
+    if (tid == 0) L.n = L.bin_end = L.bin_lo = L.bin_hi = 0;
+    float max = -INFINITY, min = INFINITY;
+    H.template each<4>([&](float f, int) {
+        max = fmaxf(max, f);                             // (a NaN is passed over)
+        min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
+    });
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            max = fmaxf(max, __shfl_xor(max, d));
-            min = fminf(min, __shfl_xor(min, d));
-        }
-        __syncthreads();                                     // (the previous row's use of LDS is over)
-        if ((tid & 63) == 0) {
-            L.max[wave] = max;
-            L.min[wave] = min;
-        }
-        if (tid == 0) L.n = L.bin_end = L.bin_lo = L.bin_hi = 0;
-        for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
+    for (int d = 32; d > 0; d >>= 1) {
+        max = fmaxf(max, __shfl_xor(max, d));
+        min = fminf(min, __shfl_xor(min, d));
+    }
+    if ((tid & 63) == 0) {
+        L.max[wave] = max;
+        L.min[wave] = min;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < BT / 64; w++) {
+        max = fmaxf(max, L.max[w]);
+        min = fminf(min, L.min[w]);
+    }
+    max = uniform(max);
+    min = uniform(min);
+    if (max == -INFINITY) {
+        if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
+        return;
+    }
+    if (r.greedy) {                                      // the first token with the largest logit
+        uint32_t at = 0xFFFFFFFFu;
+        H.template each<4>([&](float f, int i) { at = ::min(at, f == max ? (uint32_t)i : 0xFFFFFFFFu); });
+        if (tid == 0) L.last = 0xFFFFFFFFu;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < BT / 64; w++) {
-            max = fmaxf(max, L.max[w]);
-            min = fminf(min, L.min[w]);
-        }
-        if (max == -INFINITY) {
-            if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
-            continue;
-        }
-        const RowParams r = row_params(P, row);
-        if (r.greedy) {
-            __syncthreads();                                 // (from here LDS is the other search's)
-            const int64_t at = Row<BT>::template locate<DT>(shared.radix, x, V, own_key<DT>(max), 0);
-            if (tid == 0) sample_put<DT>(P, row, at, 0.0);
-            continue;
-        }
-        if (max == INFINITY || max == min) {
-            __syncthreads();
-            radix_row<DT, BT>(shared.radix, P, row, r, own_key<DT>(max));
-            continue;
-        }
-        const Weights<VQA_F32> W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
-        const double range = fmin((double)max - (double)min, WINDOW * r.t);
-        const Steps S = {(double)max, (BINS - 1) / range};
+        if (at != 0xFFFFFFFFu) atomicMin(&L.last, at);
+        __syncthreads();
+        if (tid == 0) sample_put<DT>(P, row, L.last, 0.0);
+        return;
+    }
+    if (max == INFINITY || max == min) {
+        if (tid == 0) P.token[row * P.ld_token] = LATER;
+        return;
+    }
+    const Weights<VQA_F32> W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
+    const double range = uniform(fmin((double)max - (double)min, WINDOW * r.t));
+    const Steps S = {uniform((double)max), uniform((BINS - 1) / range)};
+    float lo = min;
+    if (r.min_p > 0.0 || (double)max - (double)min > range) {
         if (wave == 0) {
             const float f = first_float(min, max, [&](float f) {
                 return (double)max - (double)f <= range && ((double)f - W.max) * W.inv_t >= W.min_z;
@@ -711,92 +776,91 @@ template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_ke
             if (tid == 0) L.lo = f;
         }
         __syncthreads();
-        const float lo = L.lo;
-        double v[BINS / BT], total = 0.0;
-        int k = r.k;
-        if (k > 0) {
-            R::each(x, V, [&](float f, int) {
-                if (f >= lo) atomicAdd(&B.cnt[S.bin(f)], 1u);
-            });
-            __syncthreads();
-            total = R::scan_bins(B, L.part, v, [&](int b) { return (double)B.cnt[b]; });
-            if (total <= (double)k) {                        // (the rest, if there is any, weighs nothing)
-                k = 0;
-                __syncthreads();
-                for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
-                __syncthreads();
-            }
-        }
-        const bool by_count = k > 0;
-        if (by_count) {
-            R::last_bin(B, v, &L.bin_hi, (double)k, false);
-        } else {
-            const double d = W.inv_t / S.scale;              // a step of the bins in z
-            const double c1 = -d, c2 = d * d / 2, c3 = -d * d * d / 6, c4 = d * d * d * d / 24, one = 1.0 + W.magic;
-            const long long magic = __double_as_longlong(W.magic);
-            R::each(x, V, [&](float f, int) {
-                if (!(f >= lo)) return;
-                const double a = S.at(f), whole = a + 4503599627370496.0, e = a - (whole - 4503599627370496.0);
-                const double p = fma(e, fma(e, fma(e, fma(e, c4, c3), c2), c1), one);
-                atomicAdd(&B.mass[(uint32_t)__double_as_longlong(whole)], (unsigned long long)(__double_as_longlong(p) - magic));
-            });
-            __syncthreads();
-            total = R::scan_bins(B, L.part, v, [&](int b) {
-                const unsigned long long m = B.mass[b];
-                return m ? ldexp((double)m, -P.shift) * exp(-d * b) : 0.0;
-            });
-            if (r.nucleus) {
-                R::last_bin(B, v, &L.bin_end, r.top_p * total, false);
-                __syncthreads();
-                if (tid == (int)L.bin_end / (BINS / BT)) {
-                    double m = 0.0;
-#pragma unroll
-                    for (int q = 0; q < BINS / BT; q++) m = q == (int)L.bin_end % (BINS / BT) ? v[q] : m;
-                    L.behind = B.front[L.bin_end] + m;
-                }
-                __syncthreads();
-                R::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
-                R::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
-            } else {
-                R::last_bin(B, v, &L.bin_lo, r.u * total, true);
-            }
-        }
-        __syncthreads();
-        // the tokens with edge 0 <= x < edge 1 or edge 2 <= x < edge 3 go on the list
-        if (wave < 4) {
-            const uint32_t end = L.bin_end;
-            const uint32_t first = by_count ? 0 : wave < 2 ? L.bin_lo : end;
-            const uint32_t last = by_count ? L.bin_hi : wave >= 2 ? end : r.nucleus ? ::min(L.bin_hi, end) : first;
-            float e = INFINITY;
-            if (!(wave & 1)) e = first_float(lo, max, [&](float f) { return S.bin(f) <= last; });
-            else if (first > 0) e = first_float(lo, max, [&](float f) { return S.bin(f) < first; });
-            if (wave >= 2 && (by_count || !r.nucleus)) e = INFINITY;
-            if ((tid & 63) == 0) L.edge[wave] = e;
-        }
-        __syncthreads();
-        const float e0 = L.edge[0], e1 = L.edge[1], e2 = L.edge[2], e3 = L.edge[3];
-        R::each(x, V, [&](float f, int i) {
-            if ((f >= e0 && f < e1) || (f >= e2 && f < e3)) {
-                const uint32_t at = atomicAdd(&L.n, 1u);
-                if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), i);
-            }
+        lo = uniform(L.lo);
+    }
+    double v[PER], total = 0.0;
+    const bool by_count = r.k > 0 && r.k < P.V;
+    if (by_count) {
+        H.template each<2>([&](float f, int) {
+            if (f >= lo) atomicAdd(&B.cnt[S.bin(f)], 1u);
         });
         __syncthreads();
-        int n = (int)L.n;
-        if (n > LIST) {
-            __syncthreads();
-            radix_row<DT, BT>(shared.radix, P, row, r, own_key<DT>(max));
-            continue;
+#pragma unroll
+        for (int q = 0; q < PER; q++) v[q] = (double)B.cnt[tid * PER + q];
+        total = BinScan<BT>::scan(B, L.part, v);
+        BinScan<BT>::last_bin(B, v, &L.bin_hi, (double)r.k, false);      // (or the last bin, where fewer tokens count)
+    } else {
+        const double d = uniform(W.inv_t / S.scale);     // a step of the bins in z
+        const double c1 = -d, c2 = uniform(d * d * 0.5), c3 = uniform(d * d * d * (-1.0 / 6.0));
+        const double c4 = uniform(d * d * d * d * (1.0 / 24.0)), one = uniform(1.0 + W.magic);
+        const long long magic = __double_as_longlong(W.magic);
+        H.template each<2>([&](float f, int) {
+            if (!(f >= lo)) return;
+            const double a = S.at(f), whole = a + 4503599627370496.0, e = a - (whole - 4503599627370496.0);
+            const double p = fma(e, fma(e, fma(e, fma(e, c4, c3), c2), c1), one);
+            atomicAdd(&B.mass[(uint32_t)__double_as_longlong(whole)], (unsigned long long)(__double_as_longlong(p) - magic));
+        });
+        __syncthreads();
+        double scale = ldexp(exp(-d * (tid * PER)), -P.shift);           // 2^-s e^(-b d) for the thread's first bin
+        const double step = exp(-d);
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            v[q] = (double)B.mass[tid * PER + q] * scale;
+            scale *= step;
         }
-        sort_list<BT>(L.list, n);
-        if (by_count && k < n) n = k;
-        finish_list<DT, BT, LIST>(L, P, row, r, W, n, by_count ? nullptr : B.front, S, total);
+        total = BinScan<BT>::scan(B, L.part, v);
+        if (r.nucleus) {
+            BinScan<BT>::last_bin(B, v, &L.bin_end, r.top_p * total, false);
+            __syncthreads();
+            if (tid == (int)L.bin_end / PER) {
+                double g = B.front[tid * PER];
+#pragma unroll
+                for (int q = 0; q < PER; q++)
+                    if (q <= (int)L.bin_end % PER) g += v[q];
+                L.behind = g;
+            }
+            __syncthreads();
+            BinScan<BT>::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
+            BinScan<BT>::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
+        } else {
+            BinScan<BT>::last_bin(B, v, &L.bin_lo, r.u * total, true);
+        }
     }
+    __syncthreads();
+    // the tokens with edge 0 <= x < edge 1 or edge 2 <= x < edge 3 go on the list
+    if (wave < 4) {
+        const uint32_t end = L.bin_end;
+        const uint32_t first = by_count ? 0 : wave < 2 ? L.bin_lo : end;
+        const uint32_t last = by_count ? L.bin_hi : wave >= 2 ? end : r.nucleus ? ::min(L.bin_hi, end) : first;
+        float e = INFINITY;
+        if (wave < 2 || (r.nucleus && !by_count)) {
+            if (!(wave & 1)) e = first_float(lo, max, [&](float f) { return S.bin(f) <= last; });
+            else if (first > 0) e = first_float(lo, max, [&](float f) { return S.bin(f) < first; });
+        }
+        if ((tid & 63) == 0) L.edge[wave] = e;
+    }
+    __syncthreads();
+    const float e0 = uniform(L.edge[0]), e1 = uniform(L.edge[1]), e2 = uniform(L.edge[2]), e3 = uniform(L.edge[3]);
+    H.template each<2>([&](float f, int i) {
+        if ((f >= e0 && f < e1) || (f >= e2 && f < e3)) {
+            const uint32_t at = atomicAdd(&L.n, 1u);
+            if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), i);
+        }
+    });
+    __syncthreads();
+    int n = (int)L.n;
+    if (n > LIST) {
+        if (tid == 0) P.token[row * P.ld_token] = LATER;
+        return;
+    }
+    const bool swapped = sort_list<BT>(L.list, L.other, n);
+    if (by_count && r.k < n) n = r.k;
+    finish_list<DT, BT, LIST>(L, swapped, P, row, r, W, n, by_count ? nullptr : B.front, S, total);
 }
 
 extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     const int size = p && p->dtype == VQA_F32 ? 4 : 2;
-    if (!p || p->rows < 0 || p->V <= 0 || p->V > 1 << 30 || !rows_dtype_ok(p->dtype) || p->ld < 0 ||
+    if (!p || p->rows < 0 || p->V <= 0 || p->V > 1 << 30 || p->rows > (int64_t)GRID_X * 65535 || !rows_dtype_ok(p->dtype) || p->ld < 0 ||
         (p->rows > 0 && (!p->logits || !p->u || !p->token)) || (uintptr_t)p->logits % size || (uintptr_t)p->token % 8 ||
         (uintptr_t)p->u % 4 || (uintptr_t)p->temperature % 4 || (uintptr_t)p->top_k % 4 || (uintptr_t)p->top_p % 4 ||
         (uintptr_t)p->min_p % 4 || (uintptr_t)p->logp % 4) {
@@ -831,12 +895,15 @@ extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
         hipLaunchKernelGGL(sample_wave_kernel<DT>, dim3((unsigned)(wg < 65536 ? wg : 65536)), dim3(256), 0, s, P);        \
     } else if (p->V <= LIST_ALL) {                                                                                        \
         hipLaunchKernelGGL((sample_list_kernel<DT, 256>), rows_grid, dim3(256), 0, s, P);                                  \
-    } else if (p->rows <= 256) {                                                                                          \
-        hipLaunchKernelGGL((sample_row_kernel<DT, 1024>), rows_grid, dim3(1024), 0, s, P);                                 \
     } else {                                                                                                              \
-        hipLaunchKernelGGL((sample_row_kernel<DT, 512>), rows_grid, dim3(512), 0, s, P);                                   \
+        const bool half = getenv("HALF") && p->rows > 256;                              \
+        if (half) hipLaunchKernelGGL((sample_row_kernel<DT, 512>), rows_grid, dim3(512), 0, s, P);                        \
+        else hipLaunchKernelGGL((sample_row_kernel<DT, 1024>), rows_grid, dim3(1024), 0, s, P);                           \
+        ROWS_CHECK_LAUNCH("vqa_sample");                                                                                  \
+        hipLaunchKernelGGL((sample_radix_kernel<DT, 1024>), later_grid, dim3(1024), 0, s, P);                             \
     }
-    const dim3 rows_grid((unsigned)(p->rows < 65536 ? p->rows : 65536));
+    const dim3 later_grid((unsigned)(p->rows < 256 ? p->rows : 256));
+    const dim3 rows_grid((unsigned)(p->rows < GRID_X ? p->rows : GRID_X), (unsigned)((p->rows + GRID_X - 1) / GRID_X));
     if (p->dtype == VQA_BF16) { SAMPLE_LAUNCH(VQA_BF16) }
     else if (p->dtype == VQA_F16) { SAMPLE_LAUNCH(VQA_F16) }
     else { SAMPLE_LAUNCH(VQA_F32) }
