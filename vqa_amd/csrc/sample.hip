@@ -16,7 +16,6 @@
 // (2^-22) one row in ten of a flat distribution over 10^5 tokens would get a neighbouring token.
 #include "rows.h"
 #include <float.h>
-#include <stdlib.h>
 
 // a bin or a comparison has to come out the same wherever it is computed: no sums fused into products but by fma()
 #pragma clang fp contract(off)
@@ -409,20 +408,15 @@ template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_radix_ker
 // The list (key and index of each token, LIST at most) is sorted in LDS, its weights are added up in order, and nucleus and
 // draw are looked up in it.  Rows whose list would be too long - many equal logits - go to the radix search.
 #define LIST_ALL 1024
-#define LIST 2048
-#define BINS 4096
 #define WINDOW 40.0
 
 typedef Keys<VQA_F32> FKeys;       // the list's keys: of the logits as fp32, whatever their type
 
-// Steps of x below the maximum: bin b holds the x with rint((max - x) scale) = b.
+// Steps of x below the maximum: bin b holds the x with floor(at(x)) = b, at(x) = (max - x) scale + 1/2.
 struct Steps {
-    double max, scale;
-    __device__ __forceinline__ double at(float x) const { return (max - (double)x) * scale; }
-    static __device__ __forceinline__ uint32_t nearest(double a) {        // 0 <= a < 2^31
-        return (uint32_t)__double_as_longlong(a + 4503599627370496.0);
-    }
-    __device__ __forceinline__ uint32_t bin(float x) const { return nearest(at(x)); }
+    double max, scale;             // (the difference first: max * scale may dwarf the 1/2)
+    __device__ __forceinline__ double at(float x) const { return fma(max - (double)x, scale, 0.5); }
+    __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)at(x); }
 };
 
 // One wave: the smallest float in [bottom, top] that `in` holds for; it holds for `top`, and for every float above one that
@@ -456,7 +450,7 @@ template <int CAP> struct ListShared {
     float max[16], min[16], edge[4], lo;
     uint32_t n, last, pick, bin_end, bin_lo, bin_hi;
 };
-union BinShared {
+template <int BINS> union BinShared {
     unsigned long long mass[BINS];
     uint32_t cnt[BINS];
     double front[BINS];                  // the weight in front of each bin
@@ -685,10 +679,10 @@ template <int DT, int BT> struct RowPass {
     }
 };
 
-template <int BT> struct BinScan {
+template <int BT, int BINS> struct BinScan {
     static constexpr int PER = BINS / BT;
     // front[b]: the sum of v over the bins before b; v: the thread's bins, read from where front goes
-    static __device__ __forceinline__ double scan(BinShared& B, double* part, const double (&v)[PER]) {
+    static __device__ __forceinline__ double scan(BinShared<BINS>& B, double* part, const double (&v)[PER]) {
         double sum = 0.0, total;
 #pragma unroll
         for (int k = 0; k < PER; k++) sum += v[k];
@@ -701,7 +695,7 @@ template <int BT> struct BinScan {
         return total;
     }
     // the last bin with something in it that starts in front of (or, `upto`, at) t
-    static __device__ __forceinline__ void last_bin(const BinShared& B, const double (&v)[PER], uint32_t* out, double t, bool upto) {
+    static __device__ __forceinline__ void last_bin(const BinShared<BINS>& B, const double (&v)[PER], uint32_t* out, double t, bool upto) {
         int mine = 0;
 #pragma unroll
         for (int k = 0; k < PER; k++) {
@@ -712,11 +706,11 @@ template <int BT> struct BinScan {
     }
 };
 
-template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_kernel(SampleArgs P) {
+template <int DT, int BT, int BINS, int LIST> __global__ __launch_bounds__(BT, 4) void sample_row_kernel(SampleArgs P) {
     typedef typename Elem<DT>::type T;
     constexpr int PER = BINS / BT;
     __shared__ ListShared<LIST> L;
-    __shared__ BinShared B;
+    __shared__ BinShared<BINS> B;
     const int tid = threadIdx.x, wave = tid >> 6;
     const int64_t row = grid_row();
     if (row >= P.rows) return;
@@ -766,7 +760,7 @@ template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_ke
     }
     const Weights<VQA_F32> W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
     const double range = uniform(fmin((double)max - (double)min, WINDOW * r.t));
-    const Steps S = {uniform((double)max), uniform((BINS - 1) / range)};
+    const Steps S = {W.max, uniform((BINS - 1) / range)};
     float lo = min;
     if (r.min_p > 0.0 || (double)max - (double)min > range) {
         if (wave == 0) {
@@ -787,30 +781,33 @@ template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_ke
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < PER; q++) v[q] = (double)B.cnt[tid * PER + q];
-        total = BinScan<BT>::scan(B, L.part, v);
-        BinScan<BT>::last_bin(B, v, &L.bin_hi, (double)r.k, false);      // (or the last bin, where fewer tokens count)
+        total = BinScan<BT, BINS>::scan(B, L.part, v);
+        BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, (double)r.k, false);      // (or the last bin, where fewer tokens count)
     } else {
         const double d = uniform(W.inv_t / S.scale);     // a step of the bins in z
-        const double c1 = -d, c2 = uniform(d * d * 0.5), c3 = uniform(d * d * d * (-1.0 / 6.0));
-        const double c4 = uniform(d * d * d * d * (1.0 / 24.0)), one = uniform(1.0 + W.magic);
+        // e^(-(f - 1/2) d) for 0 <= f < 1: the series around 1/2, in powers of f (and `magic` on top)
+        const double c1 = -d, c2 = d * d * 0.5, c3 = d * d * d * (-1.0 / 6.0), c4 = d * d * d * d * (1.0 / 24.0);
+        const double a3 = uniform(c3 - 2.0 * c4), a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4);
+        const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4);
+        const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 + W.magic);
         const long long magic = __double_as_longlong(W.magic);
         H.template each<2>([&](float f, int) {
             if (!(f >= lo)) return;
-            const double a = S.at(f), whole = a + 4503599627370496.0, e = a - (whole - 4503599627370496.0);
-            const double p = fma(e, fma(e, fma(e, fma(e, c4, c3), c2), c1), one);
-            atomicAdd(&B.mass[(uint32_t)__double_as_longlong(whole)], (unsigned long long)(__double_as_longlong(p) - magic));
+            const double a = S.at(f), e = __builtin_amdgcn_fract(a);
+            const double p = fma(e, fma(e, fma(e, fma(e, c4, a3), a2), a1), a0);
+            atomicAdd(&B.mass[(uint32_t)a], (unsigned long long)(__double_as_longlong(p) - magic));
         });
         __syncthreads();
-        double scale = ldexp(exp(-d * (tid * PER)), -P.shift);           // 2^-s e^(-b d) for the thread's first bin
+        double weight = ldexp(exp(-d * (tid * PER)), -P.shift);          // 2^-s e^(-b d) for the thread's first bin
         const double step = exp(-d);
 #pragma unroll
         for (int q = 0; q < PER; q++) {
-            v[q] = (double)B.mass[tid * PER + q] * scale;
-            scale *= step;
+            v[q] = (double)B.mass[tid * PER + q] * weight;
+            weight *= step;
         }
-        total = BinScan<BT>::scan(B, L.part, v);
+        total = BinScan<BT, BINS>::scan(B, L.part, v);
         if (r.nucleus) {
-            BinScan<BT>::last_bin(B, v, &L.bin_end, r.top_p * total, false);
+            BinScan<BT, BINS>::last_bin(B, v, &L.bin_end, r.top_p * total, false);
             __syncthreads();
             if (tid == (int)L.bin_end / PER) {
                 double g = B.front[tid * PER];
@@ -820,10 +817,10 @@ template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_ke
                 L.behind = g;
             }
             __syncthreads();
-            BinScan<BT>::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
-            BinScan<BT>::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
+            BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
+            BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
         } else {
-            BinScan<BT>::last_bin(B, v, &L.bin_lo, r.u * total, true);
+            BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * total, true);
         }
     }
     __syncthreads();
@@ -842,7 +839,7 @@ template <int DT, int BT> __global__ __launch_bounds__(BT, 4) void sample_row_ke
     __syncthreads();
     const float e0 = uniform(L.edge[0]), e1 = uniform(L.edge[1]), e2 = uniform(L.edge[2]), e3 = uniform(L.edge[3]);
     H.template each<2>([&](float f, int i) {
-        if ((f >= e0 && f < e1) || (f >= e2 && f < e3)) {
+        if (((f >= e0) & (f < e1)) | ((f >= e2) & (f < e3))) {
             const uint32_t at = atomicAdd(&L.n, 1u);
             if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), i);
         }
@@ -896,9 +893,9 @@ extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     } else if (p->V <= LIST_ALL) {                                                                                        \
         hipLaunchKernelGGL((sample_list_kernel<DT, 256>), rows_grid, dim3(256), 0, s, P);                                  \
     } else {                                                                                                              \
-        const bool half = getenv("HALF") && p->rows > 256;                              \
-        if (half) hipLaunchKernelGGL((sample_row_kernel<DT, 512>), rows_grid, dim3(512), 0, s, P);                        \
-        else hipLaunchKernelGGL((sample_row_kernel<DT, 1024>), rows_grid, dim3(1024), 0, s, P);                           \
+        if (p->rows <= 256) hipLaunchKernelGGL((sample_row_kernel<DT, 1024, 4096, 2048>), rows_grid, dim3(1024), 0, s, P); \
+        else if (p->V <= 16384) hipLaunchKernelGGL((sample_row_kernel<DT, 256, 1024, 1024>), rows_grid, dim3(256), 0, s, P); \
+        else hipLaunchKernelGGL((sample_row_kernel<DT, 512, 4096, 2048>), rows_grid, dim3(512), 0, s, P);                 \
         ROWS_CHECK_LAUNCH("vqa_sample");                                                                                  \
         hipLaunchKernelGGL((sample_radix_kernel<DT, 1024>), later_grid, dim3(1024), 0, s, P);                             \
     }
