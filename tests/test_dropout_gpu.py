@@ -140,3 +140,15 @@ def test_advancing_the_seed_tensor_before_backward_is_refused():
     state[1:].add_(7)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         y.sum().backward()
+
+
+def test_a_second_derivative_is_refused():
+    from vqa_amd.dropout import dropout
+    from vqa_amd.loss import token_log_probs
+    x = data((4, 50), 1, torch.float32).requires_grad_(True)
+    tk = torch.zeros(4, dtype=torch.int64, device=dev())
+    for y in (dropout(x, 0.5, 1), token_log_probs(x, tk)):
+        dy = torch.ones_like(y).requires_grad_(True)
+        (dx,) = torch.autograd.grad(y, x, dy, create_graph=True)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            dx.sum().backward()

@@ -31,21 +31,28 @@ def threshold(p):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, thr, seed, offset, state):
-        xc = x.detach().contiguous()
-        y = torch.empty_like(xc)
-        ops.dropout(xc, y, thr, seed, offset, state)
-        ctx.args = thr, seed, offset
-        ctx.save_for_backward(state)          # (changed before backward, it would give another mask: autograd refuses that)
+        x = x.contiguous()
+        y = torch.empty_like(x)
+        ctx.call = ops.dropout(x, y, thr, seed, offset, state)
+        if state is not None:
+            ctx.save_for_backward(state)      # (changed before backward, it would give another mask: autograd refuses that)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        (state,) = ctx.saved_tensors
-        dyc = dy.contiguous()
-        dx = torch.empty_like(dyc)
-        ops.dropout(dyc, dx, *ctx.args, state)
-        return dx, None, None, None, None
+        return (_dropout_grad_once if torch.is_grad_enabled() else _dropout_grad)(ctx, dy)
+
+
+def _dropout_grad(ctx, dy):
+    # (as little as can be: what runs in autograd's thread takes three times as long as in the caller's)
+    ctx.saved_tensors
+    dy = dy.contiguous()
+    dx = torch.empty_like(dy)
+    ops.dropout_again(dy, dx, ctx.call)
+    return dx, None, None, None, None
+
+
+_dropout_grad_once = once_differentiable(_dropout_grad)
 
 
 def dropout(x, p, seed, offset=0):

@@ -54,32 +54,35 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature, ignore, want_entropy):
         ctx.set_materialize_grads(False)
-        V = logits.size(-1)
-        x, *layout = ops.row_layout(logits.detach())
+        x, *layout = ops.row_layout(logits)
         tk = tokens.contiguous()
-        f32 = dict(dtype=torch.float32, device=x.device)
-        lp = torch.empty(tokens.shape, **f32)
-        ent = torch.empty(tokens.shape, **f32) if want_entropy else None
-        stats = torch.empty(layout[0], 4, **f32)
-        if layout[0]:
-            ops.token_logp(x, layout, tk, lp, ent, stats, V, temperature, ignore)
+        lp = torch.empty(tokens.shape, dtype=torch.float32, device=x.device)
+        ent = torch.empty_like(lp) if want_entropy else None
+        stats = torch.empty(layout[0], 4, dtype=torch.float32, device=x.device)
+        ctx.call = ops.token_logp(x, layout, tk, lp, ent, stats, x.size(-1), temperature, ignore) if layout[0] else None
         # (the caller's own tensor where it was read in place: autograd then notices a change before backward)
-        ctx.save_for_backward(logits if x.data_ptr() == logits.data_ptr() else x, tk, stats)
-        ctx.args = layout, V, temperature, ignore
+        ctx.save_for_backward(x, tk, stats)
+        ctx.like = logits.shape, x.dtype, x.device
         return (lp, ent) if want_entropy else lp
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g, h=None):
-        x, tk, stats = ctx.saved_tensors
-        layout, V, temperature, ignore = ctx.args
-        if g is None and h is None:
-            return None, None, None, None, None
-        dx = torch.empty(tuple(tk.shape) + (V,), dtype=x.dtype, device=x.device)
-        if layout[0]:
-            g, h = (t.contiguous() if t is not None else None for t in (g, h))
-            ops.token_logp_backward(x, layout, tk, stats, g, h, dx, V, temperature, ignore)
-        return dx, None, None, None, None
+        return (_log_probs_grad_once if torch.is_grad_enabled() else _log_probs_grad)(ctx, g, h)
+
+
+def _log_probs_grad(ctx, g, h):
+    # (as little as can be: what runs in autograd's thread takes three times as long as in the caller's)
+    ctx.saved_tensors
+    if g is None and h is None:
+        return None, None, None, None, None
+    shape, dtype, device = ctx.like
+    dx = torch.empty(shape, dtype=dtype, device=device)
+    if ctx.call is not None:
+        ops.token_logp_backward(ctx.call, g if g is None else g.contiguous(), h if h is None else h.contiguous(), dx)
+    return dx, None, None, None, None
+
+
+_log_probs_grad_once = once_differentiable(_log_probs_grad)
 
 
 def token_log_probs(logits, tokens, temperature=1.0, ignore_index=None, entropy=False):
