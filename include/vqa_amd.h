@@ -515,6 +515,7 @@ typedef struct {
     const float* min_p;
     int64_t* token;             /* out: token[r * ld_token] */
     float* logp;                /* out [rows], or null */
+    void* workspace;            /* vqa_sample_workspace bytes, 8-byte aligned; may be null where that is 0 */
     int64_t ld, ld_token, rows;
     double temperature_value, top_p_value, min_p_value;
     int32_t top_k_value, V;
@@ -522,6 +523,8 @@ typedef struct {
     int32_t reserved;
 } vqa_sample_params;
 
+/* bytes of workspace (few long rows are split over several workgroups) */
+int64_t vqa_sample_workspace(int64_t rows, int32_t V);
 int vqa_sample(const vqa_sample_params* p, void* stream);
 
 /* ------------------------------------------------------------------------------------------

@@ -125,9 +125,11 @@ def test_c_entry_refusals():
     for kw in (dict(logits=None), dict(u=None), dict(token=None), dict(rows=-1), dict(V=0), dict(V=2 ** 30 + 1), dict(dtype=3),
                dict(logits=0x1002), dict(token=0x1004), dict(u=0x1002), dict(top_k=0x1002), dict(logp=0x1001), dict(ld=-1)):
         _refused(lib.vqa_sample(params(**kw), None), 'vqa_sample')
+    assert lib.vqa_sample_workspace(2, 100000) > 0 and lib.vqa_sample_workspace(1000, 100000) == 0
+    _refused(lib.vqa_sample(params(rows=2, V=100000, ld=100000), None), 'vqa_sample')          # few long rows need a workspace
     assert lib.vqa_sample(params(rows=0, logits=None), None) == 0
 
 
 def test_struct_matches_the_header():
-    assert C.sizeof(_lib.SampleParams) == 8 * 8 + 3 * 8 + 3 * 8 + 4 * 4
+    assert C.sizeof(_lib.SampleParams) == 9 * 8 + 3 * 8 + 3 * 8 + 4 * 4
     assert np.dtype('f8').itemsize == 8

@@ -93,7 +93,7 @@ def test_filters(dtype, rows, V, params):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [44, 700, 9000])
+@pytest.mark.parametrize('V', [44, 700, 9000, 36000])
 def test_every_row_its_own_parameters(dtype, V):
     rows = 48
     g = torch.Generator().manual_seed(V)
@@ -116,7 +116,7 @@ def test_parameters_outside_their_range_in_a_tensor(V):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [44, 64, 300, 9001])
+@pytest.mark.parametrize('V', [44, 64, 300, 9001, 40009])
 def test_masks_infinities_and_nan(dtype, V):
     x = logits(12, V, V, dtype)
     x[0, :] = -math.inf
@@ -137,7 +137,7 @@ def test_masks_infinities_and_nan(dtype, V):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [50, 1000, 10000])
+@pytest.mark.parametrize('V', [50, 1000, 10000, 33000])
 def test_ties_go_by_index(dtype, V):
     """Constant rows and rows of two values: the cut of top-k and top-p falls among equals."""
     x = torch.zeros(4, V, dtype=dtype, device=dev())
@@ -188,9 +188,23 @@ def test_more_rows_than_workgroups():
     check(x[:64], u[:64].cpu())
 
 
+@pytest.mark.parametrize('V', [2000, 20000, 33333])
+def test_the_same_row_in_batches_of_every_size(V):
+    """How many rows a call has decides how a row is split and by how many threads it is done: the answers agree."""
+    from vqa_amd.sampling import sample
+    x = logits(300, V, V, torch.float32)
+    u = uniform(300, V).to(dev())
+    for params in (dict(top_p=0.9), dict(top_k=30), dict(temperature=0.5)):
+        want = sample(x, u, return_log_probs=True, **params)
+        for n in (1, 60, 129, 256):
+            got = sample(x[:n], u[:n], return_log_probs=True, **params)
+            assert torch.equal(got[0], want[0][:n])
+            assert ((got[1] - want[1][:n]).abs() <= want[1][:n].abs() * 2.0 ** -23).all()
+
+
 def test_another_stream_and_a_captured_graph():
     from vqa_amd.sampling import sample
-    for V in (44, 5000, 20000):
+    for V in (44, 5000, 20000, 40000):
         x = logits(6, V, V, torch.float32)
         u = uniform(6, V).to(dev())
         want = sample(x, u, top_p=0.8, return_log_probs=True)
@@ -225,7 +239,7 @@ def test_a_lone_token_has_log_probability_zero():
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [1025, 5000, 30011])
+@pytest.mark.parametrize('V', [1025, 5000, 30011, 50021])
 def test_lists_of_every_length(dtype, V):
     """Around the capacity of the list of candidates (2048): top-k beyond it, many equal logits at the cut, a bin edge that
     falls on 0 (symmetric rows), rows far from 0, tiny and huge spreads."""

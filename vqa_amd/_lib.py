@@ -68,7 +68,7 @@ class DevschedParams(C.Structure):
 
 
 class SampleParams(C.Structure):
-    _fields_ = [(n, vp) for n in ('logits', 'u', 'temperature', 'top_k', 'top_p', 'min_p', 'token', 'logp')] + \
+    _fields_ = [(n, vp) for n in ('logits', 'u', 'temperature', 'top_k', 'top_p', 'min_p', 'token', 'logp', 'workspace')] + \
                [(n, i64) for n in ('ld', 'ld_token', 'rows')] + \
                [(n, C.c_double) for n in ('temperature_value', 'top_p_value', 'min_p_value')] + \
                [(n, i32) for n in ('top_k_value', 'V', 'dtype', 'reserved')]
@@ -136,6 +136,7 @@ SIGNATURES = {
     'vqa_head_backward_workspace': (i64, [i32, i32, i32]),
     'vqa_head_backward': (i32, [vp, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i32, i32, i32, vp]),
     'vqa_xent': (i32, [vp, vp, vp, vp, vp, i32, i32, vp]),
+    'vqa_sample_workspace': (i64, [i64, i32]),
     'vqa_sample': (i32, [C.POINTER(SampleParams), vp]),
     'vqa_token_logp_workspace': (i64, [i64, i32, i32]),
     'vqa_token_logp': (i32, [vp, i64, i64, i64, vp, vp, vp, vp, vp, i64, i32, i32, C.c_float, i64, vp]),

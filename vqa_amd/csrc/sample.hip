@@ -20,6 +20,15 @@
 // a bin or a comparison has to come out the same wherever it is computed: no sums fused into products but by fma()
 #pragma clang fp contract(off)
 
+#define SPLIT_BINS 4096
+#define SPLIT_LIST 2048
+#define SPLIT_PARTS 32
+struct SplitRow {                  // see sample_row_kernel
+    unsigned long long hist[SPLIT_BINS], list[SPLIT_LIST];
+    float max[SPLIT_PARTS], min[SPLIT_PARTS];
+    uint32_t n, done;              // entries of the list; workgroups that have added theirs
+};
+
 struct SampleArgs {
     const void* x;
     int64_t ld, rows;
@@ -33,6 +42,8 @@ struct SampleArgs {
     int64_t* token;
     int64_t ld_token;
     float* logp;                   // or null
+    SplitRow* split;               // null, or a record per row
+    int32_t parts, part_size;
 };
 
 // Order-preserving keys.  Keys up to MASKED stand for -inf and NaN: tokens that are never drawn.  -0 and +0 are equal.
@@ -95,7 +106,7 @@ __device__ __forceinline__ double uniform(double v) {
     return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
 }
 
-struct RowParams { double t, top_p, min_p, u; int32_t k; bool greedy, nucleus; };
+struct RowParams { double t, top_p, min_p, u; int32_t k; bool nucleus; };
 __device__ __forceinline__ RowParams row_params(const SampleArgs& P, int64_t row) {
     RowParams r;
     r.t = uniform(P.temperature ? (double)P.temperature[row] : P.temperature_s);
@@ -104,8 +115,11 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& P, int64_t row
     r.k = P.top_k ? P.top_k[row] : P.top_k_s;
     const double u = (double)P.u[row];
     r.u = uniform(u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0);
-    r.greedy = !(r.t > 0.0);
     r.nucleus = !(r.top_p >= 1.0);
+    if (!(r.t > 0.0)) {                                      // the first token of the order
+        r.t = 1.0;
+        r.k = 1;
+    }
     return r;
 }
 template <int DT> __device__ __forceinline__ Weights<DT> row_weights(const RowParams& r, uint32_t top, int shift) {
@@ -150,11 +164,6 @@ template <int DT> __global__ __launch_bounds__(256) void sample_wave_kernel(Samp
             continue;
         }
         const RowParams r = row_params(P, row);
-        if (r.greedy) {
-            const uint64_t m = __ballot(key == top);
-            if (lane == 0) sample_put<DT>(P, row, __ffsll((unsigned long long)m) - 1, 0.0);
-            continue;
-        }
         const Weights<DT> W = row_weights<DT>(r, top, P.shift);
         const double z = key > Keys<DT>::MASKED ? W.z(key) : -INFINITY;
         const bool in = key > Keys<DT>::MASKED && z >= W.min_z;
@@ -190,18 +199,16 @@ template <int DT> __global__ __launch_bounds__(256) void sample_wave_kernel(Samp
 
 // ------------------------------------------------------------------------------------------------------------------------
 // Radix search, for any V: a workgroup of BT threads a row.
-#define RADIX_BINS 2048
-
-struct Hist {
-    uint32_t cnt[RADIX_BINS];
-    unsigned long long mass[RADIX_BINS];
+template <int RB> struct Hist {
+    uint32_t cnt[1 << RB];
+    unsigned long long mass[1 << RB];
 };
 struct Place {                     // the key that holds a place of the order
     uint32_t key;
     uint64_t cnt_above, mass_above;      // tokens and weight in front of the first token with that key
 };
-struct RadixShared {
-    Hist h1, h2;
+template <int RB> struct RadixShared {
+    Hist<RB> h1, h2;
     unsigned long long scan_c[16], scan_m[16];
     uint32_t red[16];
     uint32_t bin;
@@ -209,9 +216,11 @@ struct RadixShared {
     int64_t found;
 };
 
-template <int BT> struct Row {
+// RB: bits of the key that a level looks at
+template <int BT, int RB> struct Radix {
+    typedef RadixShared<RB> Shared;
     // the bin of `h` (of `bins` ones) that holds place t, from the top, with c / m in front of the highest bin; all threads
-    static __device__ void find_bin(RadixShared& S, const Hist& h, int bins, bool by_mass, uint64_t t, uint64_t c, uint64_t m) {
+    static __device__ void find_bin(Shared& S, const Hist<RB>& h, int bins, bool by_mass, uint64_t t, uint64_t c, uint64_t m) {
         constexpr int WAVES = BT / 64;
         const int tid = threadIdx.x, per = (bins + BT - 1) / BT;
         uint64_t sc = 0, sm = 0;
@@ -261,7 +270,7 @@ template <int BT> struct Row {
         }
         __syncthreads();
     }
-    static __device__ void clear(Hist& h, int bins) {
+    static __device__ void clear(Hist<RB>& h, int bins) {
         for (int b = threadIdx.x; b < bins; b += BT) {
             h.cnt[b] = 0;
             h.mass[b] = 0;
@@ -279,7 +288,7 @@ template <int BT> struct Row {
     }
     // histogram of (key >> shift) & (bins - 1) over the tokens that pass min-p and whose key >> up is `prefix`
     template <int DT>
-    static __device__ void count(Hist& h, const typename Elem<DT>::type* x, int V, const Weights<DT>& W, int shift, int bins,
+    static __device__ void count(Hist<RB>& h, const typename Elem<DT>::type* x, int V, const Weights<DT>& W, int shift, int bins,
                                  int up, uint32_t prefix) {
         each<DT>(x, V, [&](uint32_t key, int) {
             if (key <= Keys<DT>::MASKED || (up < 32 && (key >> up) != prefix)) return;
@@ -292,14 +301,14 @@ template <int BT> struct Row {
         });
     }
     template <int DT>
-    static __device__ Place find(RadixShared& S, const typename Elem<DT>::type* x, int V, const Weights<DT>& W, bool by_mass, uint64_t t) {
+    static __device__ Place find(Shared& S, const typename Elem<DT>::type* x, int V, const Weights<DT>& W, bool by_mass, uint64_t t) {
         constexpr int B = Keys<DT>::BITS;
         Place p;
-        find_bin(S, S.h1, RADIX_BINS, by_mass, t, 0, 0);
+        find_bin(S, S.h1, (1 << RB), by_mass, t, 0, 0);
         uint32_t prefix = S.bin;
-        int low = B - 11;                                    // bits that are still open
+        int low = B - RB;                                    // bits that are still open
         while (low > 0) {
-            const int bits = low > 11 ? 11 : low, bins = 1 << bits;
+            const int bits = low > RB ? RB : low, bins = 1 << bits;
             const uint64_t c = S.cnt_above, m = S.mass_above;
             clear(S.h2, bins);
             __syncthreads();
@@ -318,7 +327,7 @@ template <int BT> struct Row {
     // index of the (j + 1)-th token with this key: every wave counts a contiguous piece of the row, then the right one
     // looks closer
     template <int DT>
-    static __device__ int64_t locate(RadixShared& S, const typename Elem<DT>::type* x, int V, uint32_t key, uint64_t j) {
+    static __device__ int64_t locate(Shared& S, const typename Elem<DT>::type* x, int V, uint32_t key, uint64_t j) {
         constexpr int WAVES = BT / 64;
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         const int piece = ((V + WAVES - 1) / WAVES + 63) / 64 * 64;
@@ -348,30 +357,29 @@ template <int BT> struct Row {
     }
 };
 
-// The rows that sample_row_kernel left: those whose token is LATER.
-#define LATER INT64_MIN
-template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_radix_kernel(SampleArgs P) {
+// The whole answer for one row, not masked as a whole, by radix search; all threads of the workgroup.  Not inlined: rows that
+// come here are rare, and the kernels that call it keep their registers.
+template <int DT, int BT, int RB> __device__ __attribute__((noinline)) void radix_row(LDS_AS void* lds, SampleArgs P, int64_t row) {
     typedef typename Elem<DT>::type T;
-    typedef Row<BT> R;
-    __shared__ RadixShared S;
+    typedef Radix<BT, RB> R;
+    typename R::Shared& S = *(typename R::Shared*)(LDS_AS typename R::Shared*)lds;
     const int tid = threadIdx.x;
-    for (int64_t row = blockIdx.x; row < P.rows; row += gridDim.x) {
-    if (P.token[row * P.ld_token] != LATER) continue;        // (the same for all threads: it is written behind a barrier)
     const T* x = (const T*)P.x + row * P.ld;
     const RowParams r = row_params(P, row);
+    __syncthreads();                                         // (LDS was somebody else's)
     uint32_t top = 0;
     R::template each<DT>(x, P.V, [&](uint32_t key, int) { top = max(top, key); });
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     if ((tid & 63) == 0) S.red[tid >> 6] = top;
-    R::clear(S.h1, RADIX_BINS);
+    R::clear(S.h1, 1 << RB);
     __syncthreads();
     for (int w = 0; w < BT / 64; w++) top = max(top, S.red[w]);
     const Weights<DT> W = row_weights<DT>(r, top, P.shift);
-    R::template count<DT>(S.h1, x, P.V, W, Keys<DT>::BITS - 11, RADIX_BINS, 32, 0);
+    R::template count<DT>(S.h1, x, P.V, W, Keys<DT>::BITS - RB, 1 << RB, 32, 0);
     __syncthreads();
     uint64_t n = 0, total = 0;
-    for (int b = tid & 63; b < RADIX_BINS; b += 64) {        // (every wave for itself)
+    for (int b = tid & 63; b < 1 << RB; b += 64) {           // (every wave for itself)
         n += S.h1.cnt[b];
         total += S.h1.mass[b];
     }
@@ -394,7 +402,6 @@ template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_radix_ker
     const Place p = R::template find<DT>(S, x, P.V, W, true, t);
     const int64_t at = R::template locate<DT>(S, x, P.V, p.key, (t - p.mass_above) / W.of(p.key));
     if (tid == 0) sample_put<DT>(P, row, at, W.z(p.key) - log(ldexp((double)total, -P.shift)));
-    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
@@ -451,8 +458,7 @@ template <int CAP> struct ListShared {
     uint32_t n, last, pick, bin_end, bin_lo, bin_hi;
 };
 template <int BINS> union BinShared {
-    unsigned long long mass[BINS];
-    uint32_t cnt[BINS];
+    unsigned long long mass[BINS];       // weights, or the numbers of tokens
     double front[BINS];                  // the weight in front of each bin
 };
 
@@ -517,8 +523,12 @@ template <int BT> __device__ __forceinline__ bool sort_list(unsigned long long* 
                     list[b] = va;
                 }
             }
-            __syncthreads();
+            // the pairs of a wave's 64 neighbouring p are its own 128 entries while j <= 64: no other wave touches them
+            // before a step with a larger j (the next one is the next k's first)
+            if (j > 64 || (j == 1 && k >= 128)) __syncthreads();
+            else __builtin_amdgcn_wave_barrier(), __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+    __syncthreads();
     return false;
 }
 
@@ -622,11 +632,7 @@ template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_list_kern
         if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
         return;
     }
-    RowParams r = row_params(P, row);
-    if (r.greedy) {                                      // the first token of the order
-        r.t = 1.0;
-        r.k = 1;
-    }
+    const RowParams r = row_params(P, row);
     const Weights<VQA_F32> W = row_weights<VQA_F32>(r, top, P.shift);
     int mine = 0;
 #pragma unroll
@@ -706,56 +712,80 @@ template <int BT, int BINS> struct BinScan {
     }
 };
 
-template <int DT, int BT, int BINS, int LIST> __global__ __launch_bounds__(BT, 4) void sample_row_kernel(SampleArgs P) {
+// WHOLE: one workgroup does a row.  Few long rows are split over P.parts workgroups each, in three launches that meet in
+// SplitRow, a workspace per row: MAXIMUM, HISTOGRAM and COLLECT do a pass over their part each, and the workgroup that comes
+// last to the row's list does the rest.  What depends on the whole row is computed by each of its workgroups anew.
+enum SamplePhase { WHOLE, MAXIMUM, HISTOGRAM, COLLECT };
+template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __launch_bounds__(BT, 4) void sample_row_kernel(SampleArgs P) {
     typedef typename Elem<DT>::type T;
     constexpr int PER = BINS / BT;
-    __shared__ ListShared<LIST> L;
-    __shared__ BinShared<BINS> B;
+    constexpr bool SPLIT = PHASE != WHOLE;
+    constexpr int RB = BINS >= 4096 ? 11 : 10;
+    __shared__ union {
+        struct {
+            ListShared<LIST> L;
+            BinShared<BINS> B;
+        } s;
+        RadixShared<RB> radix;
+    } shared;
+    ListShared<LIST>& L = shared.s.L;
+    BinShared<BINS>& B = shared.s.B;
     const int tid = threadIdx.x, wave = tid >> 6;
-    const int64_t row = grid_row();
+    const int part = SPLIT ? blockIdx.x % P.parts : 0;
+    const int64_t row = SPLIT ? blockIdx.x / P.parts : grid_row();
     if (row >= P.rows) return;
-    const RowPass<DT, BT> H((const T*)P.x + row * P.ld, P.V);
-    const RowParams r = row_params(P, row);
-    for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
-    if (tid == 0) L.n = L.bin_end = L.bin_lo = L.bin_hi = 0;
+    SplitRow* const Q = P.split + (SPLIT ? row : 0);
+    const int first_index = part * P.part_size;
+    const RowPass<DT, BT> H((const T*)P.x + row * P.ld + first_index, SPLIT ? ::min(P.part_size, P.V - first_index) : P.V);
     float max = -INFINITY, min = INFINITY;
-    H.template each<4>([&](float f, int) {
-        max = fmaxf(max, f);                             // (a NaN is passed over)
-        min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
-    });
+    if (PHASE == WHOLE || PHASE == HISTOGRAM)
+        for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
+    if (tid == 0) L.n = L.bin_end = L.bin_lo = L.bin_hi = 0;
+    if (PHASE == WHOLE || PHASE == MAXIMUM) {
+        H.template each<4>([&](float f, int) {
+            max = fmaxf(max, f);                             // (a NaN is passed over)
+            min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
+        });
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        max = fmaxf(max, __shfl_xor(max, d));
-        min = fminf(min, __shfl_xor(min, d));
-    }
-    if ((tid & 63) == 0) {
-        L.max[wave] = max;
-        L.min[wave] = min;
-    }
-    __syncthreads();
+        for (int d = 32; d > 0; d >>= 1) {
+            max = fmaxf(max, __shfl_xor(max, d));
+            min = fminf(min, __shfl_xor(min, d));
+        }
+        if ((tid & 63) == 0) {
+            L.max[wave] = max;
+            L.min[wave] = min;
+        }
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < BT / 64; w++) {
-        max = fmaxf(max, L.max[w]);
-        min = fminf(min, L.min[w]);
+        for (int w = 0; w < BT / 64; w++) {
+            max = fmaxf(max, L.max[w]);
+            min = fminf(min, L.min[w]);
+        }
+    } else {
+        __syncthreads();
+        for (int q = 0; q < P.parts; q++) {
+            max = fmaxf(max, Q->max[q]);
+            min = fminf(min, Q->min[q]);
+        }
     }
+    if (PHASE == MAXIMUM) {
+        for (int b = part * BT + tid; b < BINS; b += P.parts * BT) Q->hist[b] = 0;
+        if (tid == 0) {
+            Q->max[part] = max;
+            Q->min[part] = min;
+            if (part == 0) Q->n = Q->done = 0;
+        }
+        return;
+    }
+    const RowParams r = row_params(P, row);
     max = uniform(max);
     min = uniform(min);
     if (max == -INFINITY) {
-        if (tid == 0) sample_put<DT>(P, row, -1, -INFINITY);
-        return;
-    }
-    if (r.greedy) {                                      // the first token with the largest logit
-        uint32_t at = 0xFFFFFFFFu;
-        H.template each<4>([&](float f, int i) { at = ::min(at, f == max ? (uint32_t)i : 0xFFFFFFFFu); });
-        if (tid == 0) L.last = 0xFFFFFFFFu;
-        __syncthreads();
-        if (at != 0xFFFFFFFFu) atomicMin(&L.last, at);
-        __syncthreads();
-        if (tid == 0) sample_put<DT>(P, row, L.last, 0.0);
+        if (tid == 0 && part == 0) sample_put<DT>(P, row, -1, -INFINITY);
         return;
     }
     if (max == INFINITY || max == min) {
-        if (tid == 0) P.token[row * P.ld_token] = LATER;
+        if (PHASE == WHOLE || (PHASE == COLLECT && part == 0)) radix_row<DT, BT, RB>((LDS_AS void*)&shared, P, row);
         return;
     }
     const Weights<VQA_F32> W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
@@ -772,56 +802,63 @@ template <int DT, int BT, int BINS, int LIST> __global__ __launch_bounds__(BT, 4
         __syncthreads();
         lo = uniform(L.lo);
     }
-    double v[PER], total = 0.0;
     const bool by_count = r.k > 0 && r.k < P.V;
-    if (by_count) {
-        H.template each<2>([&](float f, int) {
-            if (f >= lo) atomicAdd(&B.cnt[S.bin(f)], 1u);
-        });
+    const double d = uniform(W.inv_t / S.scale);         // a step of the bins in z
+    if (PHASE == WHOLE || PHASE == HISTOGRAM) {
+        if (by_count) {
+            H.template each<2>([&](float f, int) {
+                if (f >= lo) atomicAdd((uint32_t*)&B.mass[S.bin(f)], 1u);
+            });
+        } else {
+            // e^(-(f - 1/2) d) for 0 <= f < 1: the series around 1/2, in powers of f (and `magic` on top)
+            const double c1 = -d, c2 = d * d * 0.5, c3 = d * d * d * (-1.0 / 6.0), c4 = d * d * d * d * (1.0 / 24.0);
+            const double a3 = uniform(c3 - 2.0 * c4), a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4);
+            const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4);
+            const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 + W.magic);
+            const long long magic = __double_as_longlong(W.magic);
+            H.template each<2>([&](float f, int) {
+                if (!(f >= lo)) return;
+                const double a = S.at(f), e = __builtin_amdgcn_fract(a);
+                const double p = fma(e, fma(e, fma(e, fma(e, c4, a3), a2), a1), a0);
+                atomicAdd(&B.mass[(uint32_t)a], (unsigned long long)(__double_as_longlong(p) - magic));
+            });
+        }
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < PER; q++) v[q] = (double)B.cnt[tid * PER + q];
-        total = BinScan<BT, BINS>::scan(B, L.part, v);
-        BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, (double)r.k, false);      // (or the last bin, where fewer tokens count)
-    } else {
-        const double d = uniform(W.inv_t / S.scale);     // a step of the bins in z
-        // e^(-(f - 1/2) d) for 0 <= f < 1: the series around 1/2, in powers of f (and `magic` on top)
-        const double c1 = -d, c2 = d * d * 0.5, c3 = d * d * d * (-1.0 / 6.0), c4 = d * d * d * d * (1.0 / 24.0);
-        const double a3 = uniform(c3 - 2.0 * c4), a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4);
-        const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4);
-        const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 + W.magic);
-        const long long magic = __double_as_longlong(W.magic);
-        H.template each<2>([&](float f, int) {
-            if (!(f >= lo)) return;
-            const double a = S.at(f), e = __builtin_amdgcn_fract(a);
-            const double p = fma(e, fma(e, fma(e, fma(e, c4, a3), a2), a1), a0);
-            atomicAdd(&B.mass[(uint32_t)a], (unsigned long long)(__double_as_longlong(p) - magic));
-        });
-        __syncthreads();
-        double weight = ldexp(exp(-d * (tid * PER)), -P.shift);          // 2^-s e^(-b d) for the thread's first bin
-        const double step = exp(-d);
+    }
+    if (PHASE == HISTOGRAM) {
+        for (int b = tid; b < BINS; b += BT)
+            if (B.mass[b]) atomicAdd(&Q->hist[b], B.mass[b]);
+        return;
+    }
+    // the weight, or with top-k the number, of the tokens in each bin
+    double v[PER];
+    {
+        double weight = by_count ? 1.0 : ldexp(exp(-d * (tid * PER)), -P.shift);     // 2^-s e^(-b d) for the thread's first bin
+        const double step = by_count ? 1.0 : exp(-d);
 #pragma unroll
         for (int q = 0; q < PER; q++) {
-            v[q] = (double)B.mass[tid * PER + q] * weight;
+            v[q] = (double)(SPLIT ? Q->hist[tid * PER + q] : B.mass[tid * PER + q]) * weight;
             weight *= step;
         }
-        total = BinScan<BT, BINS>::scan(B, L.part, v);
-        if (r.nucleus) {
-            BinScan<BT, BINS>::last_bin(B, v, &L.bin_end, r.top_p * total, false);
-            __syncthreads();
-            if (tid == (int)L.bin_end / PER) {
-                double g = B.front[tid * PER];
+    }
+    const double total = BinScan<BT, BINS>::scan(B, L.part, v);
+    if (by_count) {
+        BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, (double)r.k, false);        // (or the last bin, where fewer tokens count)
+    } else if (r.nucleus) {
+        BinScan<BT, BINS>::last_bin(B, v, &L.bin_end, r.top_p * total, false);
+        __syncthreads();
+        if (tid == (int)L.bin_end / PER) {
+            double g = B.front[tid * PER];
 #pragma unroll
-                for (int q = 0; q < PER; q++)
-                    if (q <= (int)L.bin_end % PER) g += v[q];
-                L.behind = g;
-            }
-            __syncthreads();
-            BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
-            BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
-        } else {
-            BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * total, true);
+            for (int q = 0; q < PER; q++)
+                if (q <= (int)L.bin_end % PER) g += v[q];
+            L.behind = g;
         }
+        __syncthreads();
+        BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
+        BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, r.u * L.behind, true);
+    } else {
+        BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * total, true);
     }
     __syncthreads();
     // the tokens with edge 0 <= x < edge 1 or edge 2 <= x < edge 3 go on the list
@@ -841,26 +878,59 @@ template <int DT, int BT, int BINS, int LIST> __global__ __launch_bounds__(BT, 4
     H.template each<2>([&](float f, int i) {
         if (((f >= e0) & (f < e1)) | ((f >= e2) & (f < e3))) {
             const uint32_t at = atomicAdd(&L.n, 1u);
-            if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), i);
+            if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), first_index + i);
         }
     });
     __syncthreads();
     int n = (int)L.n;
+    if (SPLIT) {                                             // add them to the row's list; the last workgroup takes it
+        if (tid == 0) L.last = atomicAdd(&Q->n, (uint32_t)n);
+        __syncthreads();
+        // (entries as atomic stores, and one release a workgroup: a fence by every wave writes the L2 cache back each time,
+        // 43 us for 256 workgroups)
+        for (int i = tid; i < n; i += BT)
+            if (i < LIST && L.last + i < LIST)
+                __hip_atomic_store(&Q->list[L.last + i], L.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (tid == 0) L.pick = __hip_atomic_fetch_add(&Q->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if ((int)L.pick != P.parts - 1) return;
+        n = (int)__hip_atomic_load(&Q->n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     if (n > LIST) {
-        if (tid == 0) P.token[row * P.ld_token] = LATER;
+        radix_row<DT, BT, RB>((LDS_AS void*)&shared, P, row);
         return;
+    }
+    if (SPLIT) {
+        for (int i = tid; i < n; i += BT) L.list[i] = __hip_atomic_load(&Q->list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
     }
     const bool swapped = sort_list<BT>(L.list, L.other, n);
     if (by_count && r.k < n) n = r.k;
     finish_list<DT, BT, LIST>(L, swapped, P, row, r, W, n, by_count ? nullptr : B.front, S, total);
 }
 
+// Workgroups of a row.  Half of the device's 256 units are idle with 128 rows or fewer; a part keeps 8192 logits, below
+// which the four launches cost more than they save.
+static int sample_parts(int64_t rows, int32_t V) {
+    if (rows <= 0 || rows > 128 || V < 4 * 8192) return 1;
+    const int64_t by_rows = 256 / rows, by_size = V / 8192;
+    const int64_t parts = by_rows < by_size ? by_rows : by_size;
+    return (int)(parts < SPLIT_PARTS ? parts : SPLIT_PARTS);
+}
+
+extern "C" int64_t vqa_sample_workspace(int64_t rows, int32_t V) {
+    return sample_parts(rows, V) > 1 ? rows * (int64_t)sizeof(SplitRow) : 0;
+}
+
 extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     const int size = p && p->dtype == VQA_F32 ? 4 : 2;
+    const int parts = p ? sample_parts(p->rows, p->V) : 1;
     if (!p || p->rows < 0 || p->V <= 0 || p->V > 1 << 30 || p->rows > (int64_t)GRID_X * 65535 || !rows_dtype_ok(p->dtype) || p->ld < 0 ||
         (p->rows > 0 && (!p->logits || !p->u || !p->token)) || (uintptr_t)p->logits % size || (uintptr_t)p->token % 8 ||
         (uintptr_t)p->u % 4 || (uintptr_t)p->temperature % 4 || (uintptr_t)p->top_k % 4 || (uintptr_t)p->top_p % 4 ||
-        (uintptr_t)p->min_p % 4 || (uintptr_t)p->logp % 4) {
+        (uintptr_t)p->min_p % 4 || (uintptr_t)p->logp % 4 ||
+        (parts > 1 && (!p->workspace || (uintptr_t)p->workspace % 8))) {
         vqa_set_error("vqa_sample: bad argument");
         return VQA_EINVAL;
     }
@@ -882,6 +952,9 @@ extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     P.token = p->token;
     P.ld_token = p->ld_token;
     P.logp = p->logp;
+    P.split = (SplitRow*)p->workspace;
+    P.parts = parts;
+    P.part_size = ((p->V + parts - 1) / parts + 63) / 64 * 64;
     int log_v = 0;
     while (((int64_t)1 << log_v) < p->V) log_v++;
     P.shift = 62 - log_v < 51 ? 62 - log_v : 51;             // V 2^s <= 2^62; w + 2^(52 - s) does not leave its binade
@@ -893,18 +966,27 @@ extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     } else if (p->V <= LIST_ALL) {                                                                                        \
         hipLaunchKernelGGL((sample_list_kernel<DT, 256>), rows_grid, dim3(256), 0, s, P);                                  \
     } else {                                                                                                              \
-        if (p->rows <= 256) hipLaunchKernelGGL((sample_row_kernel<DT, 1024, 4096, 2048>), rows_grid, dim3(1024), 0, s, P); \
-        else if (p->V <= 16384) hipLaunchKernelGGL((sample_row_kernel<DT, 256, 1024, 1024>), rows_grid, dim3(256), 0, s, P); \
-        else hipLaunchKernelGGL((sample_row_kernel<DT, 512, 4096, 2048>), rows_grid, dim3(512), 0, s, P);                 \
-        ROWS_CHECK_LAUNCH("vqa_sample");                                                                                  \
-        hipLaunchKernelGGL((sample_radix_kernel<DT, 1024>), later_grid, dim3(1024), 0, s, P);                             \
+        if (parts > 1) {                                                                                                  \
+            SAMPLE_PHASE(DT, MAXIMUM, parts_grid)                                                                         \
+            SAMPLE_PHASE(DT, HISTOGRAM, parts_grid)                                                                       \
+            SAMPLE_PHASE(DT, COLLECT, parts_grid)                                                                         \
+        } else if (p->rows <= 256)                                                                                        \
+            hipLaunchKernelGGL((sample_row_kernel<DT, 1024, 4096, 2048, WHOLE>), rows_grid, dim3(1024), 0, s, P);         \
+        else if (p->V <= 16384)                                                                                           \
+            hipLaunchKernelGGL((sample_row_kernel<DT, 256, 1024, 1024, WHOLE>), rows_grid, dim3(256), 0, s, P);           \
+        else                                                                                                              \
+            hipLaunchKernelGGL((sample_row_kernel<DT, 512, 4096, 2048, WHOLE>), rows_grid, dim3(512), 0, s, P);           \
     }
-    const dim3 later_grid((unsigned)(p->rows < 256 ? p->rows : 256));
+    const dim3 parts_grid((unsigned)(parts > 1 ? p->rows * parts : 1));
+#define SAMPLE_PHASE(DT, PHASE, GRID)                                                                                     \
+    hipLaunchKernelGGL((sample_row_kernel<DT, 512, SPLIT_BINS, SPLIT_LIST, PHASE>), GRID, dim3(512), 0, s, P);            \
+    ROWS_CHECK_LAUNCH("vqa_sample");
     const dim3 rows_grid((unsigned)(p->rows < GRID_X ? p->rows : GRID_X), (unsigned)((p->rows + GRID_X - 1) / GRID_X));
     if (p->dtype == VQA_BF16) { SAMPLE_LAUNCH(VQA_BF16) }
     else if (p->dtype == VQA_F16) { SAMPLE_LAUNCH(VQA_F16) }
     else { SAMPLE_LAUNCH(VQA_F32) }
 #undef SAMPLE_LAUNCH
+#undef SAMPLE_PHASE
     ROWS_CHECK_LAUNCH("vqa_sample");
     return VQA_OK;
 }

@@ -363,7 +363,11 @@ def sample(x, ld, rows, V, u, token, ld_token, logp, temperature, top_k, top_p, 
     assert logp is None or (logp.dtype == torch.float32 and logp.is_contiguous() and logp.numel() == rows)
     p.logits, p.u, p.token, p.logp = x.data_ptr(), u.data_ptr(), token.data_ptr(), _addr(logp)
     p.ld, p.ld_token, p.rows, p.V, p.dtype = ld, ld_token, rows, V, ROW_DTYPES[x.dtype]
-    _call_on(x, _lib.load().vqa_sample, C.byref(p))
+    lib = _lib.load()
+    need = lib.vqa_sample_workspace(rows, V)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    p.workspace = _addr(ws)
+    _call_on(x, lib.vqa_sample, C.byref(p))
 
 
 def row_layout(x):
