@@ -170,15 +170,20 @@ template <int DT> __global__ __launch_bounds__(256) void sample_wave_kernel(Samp
         const uint64_t w = in ? W.of_z(z) : 0;
         int before = 0;
         uint64_t mass = 0;                                   // (of what stands before; tokens that are out weigh nothing)
-        for (int l = 0; l < P.V; l++) {
-            const uint32_t kl = __builtin_amdgcn_readlane(key, l);
-            const uint64_t wl = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)w, l) |
-                                ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(w >> 32), l) << 32);
-            if (kl > key || (kl == key && l < lane)) {
-                before++;
-                mass += wl;
-            }
+        const uint64_t mine = ((uint64_t)key << 32) | (uint32_t)~lane;       // larger: before
+        auto look = [&](int l) {                             // without a branch: a compare, two selects, two sums
+            const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(key, l) << 32) | (uint32_t)~l;
+            const uint64_t wl = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(w >> 32), l) << 32) |
+                                (uint32_t)__builtin_amdgcn_readlane((uint32_t)w, l);
+            before += other > mine;
+            mass += other > mine ? wl : 0;
+        };
+        int l = 0;
+        for (; l + 4 <= P.V; l += 4) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) look(l + k);
         }
+        for (; l < P.V; l++) look(l);
         auto sum = [](uint64_t v) {
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, d);
@@ -414,7 +419,7 @@ template <int DT, int BT, int RB> __device__ __attribute__((noinline)) void radi
 //   3. the list: the tokens of the bin that the nucleus ends in and of the bins that the draw can fall into.
 // The list (key and index of each token, LIST at most) is sorted in LDS, its weights are added up in order, and nucleus and
 // draw are looked up in it.  Rows whose list would be too long - many equal logits - go to the radix search.
-#define LIST_ALL 1024
+#define LIST_ALL 128
 #define WINDOW 40.0
 
 typedef Keys<VQA_F32> FKeys;       // the list's keys: of the logits as fp32, whatever their type
@@ -608,20 +613,16 @@ template <int DT> __device__ __forceinline__ uint32_t float_key(const typename E
 #define GRID_X (1 << 20)
 __device__ __forceinline__ int64_t grid_row() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
-template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_list_kernel(SampleArgs P) {
+template <int DT> __global__ __launch_bounds__(2 * LIST_ALL) void sample_list_kernel(SampleArgs P) {
     typedef typename Elem<DT>::type T;
-    constexpr int PER = LIST_ALL / BT;
+    constexpr int BT = 2 * LIST_ALL;                         // (two threads an entry: sort_list counts)
     __shared__ ListShared<LIST_ALL> L;
     const int tid = threadIdx.x, V = P.V;
     const int64_t row = grid_row();
     if (row >= P.rows) return;
     const T* x = (const T*)P.x + row * P.ld;
-    uint32_t key[PER], top = 0;
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-        key[k] = k * BT + tid < V ? float_key<DT>(x, k * BT + tid) : 0;
-        top = max(top, key[k]);
-    }
+    const uint32_t key = tid < V ? float_key<DT>(x, tid) : 0;
+    uint32_t top = key;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     if ((tid & 63) == 0) L.max[tid >> 6] = __uint_as_float(top);
@@ -634,16 +635,11 @@ template <int DT, int BT> __global__ __launch_bounds__(BT) void sample_list_kern
     }
     const RowParams r = row_params(P, row);
     const Weights<VQA_F32> W = row_weights<VQA_F32>(r, top, P.shift);
-    int mine = 0;
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-        const bool in = key[k] > FKeys::MASKED && W.z(key[k]) >= W.min_z;
-        L.list[k * BT + tid] = in ? list_entry(key[k], k * BT + tid) : 0;
-        mine += in;
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d);
-    if ((tid & 63) == 0) atomicAdd(&L.n, (uint32_t)mine);
+    const bool in = key > FKeys::MASKED && W.z(key) >= W.min_z;
+    if (tid < LIST_ALL) L.list[tid] = in ? list_entry(key, tid) : 0;
+    const uint64_t m = __ballot(in);
+    if ((tid & 63) == 0) atomicAdd(&L.n, (uint32_t)__popcll((unsigned long long)m));
+    __syncthreads();
     const bool swapped = sort_list<BT>(L.list, L.other, V);
     int n = (int)L.n;
     if (r.k > 0 && r.k < n) n = r.k;
@@ -964,13 +960,13 @@ extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
         const int64_t wg = (p->rows + 3) / 4;                                                                             \
         hipLaunchKernelGGL(sample_wave_kernel<DT>, dim3((unsigned)(wg < 65536 ? wg : 65536)), dim3(256), 0, s, P);        \
     } else if (p->V <= LIST_ALL) {                                                                                        \
-        hipLaunchKernelGGL((sample_list_kernel<DT, 256>), rows_grid, dim3(256), 0, s, P);                                  \
+        hipLaunchKernelGGL(sample_list_kernel<DT>, rows_grid, dim3(2 * LIST_ALL), 0, s, P);                               \
     } else {                                                                                                              \
         if (parts > 1) {                                                                                                  \
             SAMPLE_PHASE(DT, MAXIMUM, parts_grid)                                                                         \
             SAMPLE_PHASE(DT, HISTOGRAM, parts_grid)                                                                       \
             SAMPLE_PHASE(DT, COLLECT, parts_grid)                                                                         \
-        } else if (p->rows <= 256)                                                                                        \
+        } else if (p->rows <= 256 && p->V > 4096)                                                                         \
             hipLaunchKernelGGL((sample_row_kernel<DT, 1024, 4096, 2048, WHOLE>), rows_grid, dim3(1024), 0, s, P);         \
         else if (p->V <= 16384)                                                                                           \
             hipLaunchKernelGGL((sample_row_kernel<DT, 256, 1024, 1024, WHOLE>), rows_grid, dim3(256), 0, s, P);           \

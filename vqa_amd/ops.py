@@ -349,24 +349,22 @@ def _addr(t):
 def sample(x, ld, rows, V, u, token, ld_token, logp, temperature, top_k, top_p, min_p):
     """vqa_sample: token[r * ld_token] (and logp) of row r at element r * ld of x; the last four: a number, or one per row
     (fp32, int32 for top_k)"""
-    p = _lib.SampleParams()
-    p.temperature_value, p.top_k_value, p.top_p_value, p.min_p_value = 1.0, 0, 1.0, 0.0
-    for name, v in (('temperature', temperature), ('top_k', top_k), ('top_p', top_p), ('min_p', min_p)):
+    values, pointers = [1.0, 0, 1.0, 0.0], [None, None, None, None]
+    for i, v in enumerate((temperature, top_k, top_p, min_p)):
         if isinstance(v, torch.Tensor):
-            assert v.dtype == (torch.int32 if name == 'top_k' else torch.float32) and v.is_contiguous() and v.numel() == rows
+            assert v.dtype == (torch.int32 if i == 1 else torch.float32) and v.is_contiguous() and v.numel() == rows
             _same_device(x, v)
-            setattr(p, name, v.data_ptr())
+            pointers[i] = v.data_ptr()
         else:
-            setattr(p, name + '_value', v)
+            values[i] = v
     _same_device(x, u, token, logp)
     assert u.dtype == torch.float32 and u.is_contiguous() and u.numel() == rows and token.dtype == torch.int64
     assert logp is None or (logp.dtype == torch.float32 and logp.is_contiguous() and logp.numel() == rows)
-    p.logits, p.u, p.token, p.logp = x.data_ptr(), u.data_ptr(), token.data_ptr(), _addr(logp)
-    p.ld, p.ld_token, p.rows, p.V, p.dtype = ld, ld_token, rows, V, ROW_DTYPES[x.dtype]
     lib = _lib.load()
     need = lib.vqa_sample_workspace(rows, V)
     ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    p.workspace = _addr(ws)
+    p = _lib.SampleParams(x.data_ptr(), u.data_ptr(), *pointers, token.data_ptr(), _addr(logp), _addr(ws), ld, ld_token, rows,
+                          values[0], values[2], values[3], values[1], V, ROW_DTYPES[x.dtype], 0)
     _call_on(x, lib.vqa_sample, C.byref(p))
 
 

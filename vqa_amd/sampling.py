@@ -17,17 +17,21 @@ import torch
 from . import ops
 
 
-def _per_row(name, v, rows, x, lo, hi):
+_RANGES = dict(temperature=(0.0, 1e30), top_k=(0, 2 ** 31 - 1), top_p=(0.0, 1.0), min_p=(0.0, 1.0))
+
+
+def _per_row(name, v, rows, device):
     """A number (checked), or a tensor with one value per row in the type the kernel reads.  (Values in a tensor are not looked
     at here: that would wait for the device.  The kernel has an answer for each.)"""
-    kind = torch.int32 if name == 'top_k' else torch.float32
     if isinstance(v, torch.Tensor):
-        if v.shape != (rows,) or v.device != x.device or v.is_floating_point() != kind.is_floating_point or v.dtype == torch.bool:
+        kind = torch.int32 if name == 'top_k' else torch.float32
+        if v.shape != (rows,) or v.device != device or v.is_floating_point() != kind.is_floating_point or v.dtype == torch.bool:
             raise ValueError('%s must be a number or a tensor of %d %s on the device of the logits' %
                              (name, rows, 'integers' if name == 'top_k' else 'floating numbers'))
-        if name == 'top_k' and v.dtype == torch.int64:
-            v = v.clamp(0, hi)
-        return v.to(kind).contiguous()
+        if v.dtype == torch.int64:
+            v = v.clamp(0, _RANGES[name][1])
+        return v.detach().to(kind).contiguous()
+    lo, hi = _RANGES[name]
     v = int(v) if name == 'top_k' else float(v)
     if not lo <= v <= hi:
         raise ValueError('%s must be in [%g, %g]' % (name, lo, hi))
@@ -49,15 +53,13 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
         raise ValueError('u must be fp32 [%d]' % rows)
     if out is not None and (out.shape != (rows,) or out.dtype != torch.int64 or (rows > 1 and out.stride(0) == 0)):
         raise ValueError('out must be int64 [%d]' % rows)
-    ops._same_device(logits, u, out)
-    x = logits.detach()
-    if (V > 1 and x.stride(1) != 1):
-        x = x.contiguous()
-    params = [_per_row(*a, rows, x, lo, hi) for *a, lo, hi in (
-        ('temperature', temperature, 0.0, 1e30), ('top_k', top_k, 0, 2 ** 31 - 1), ('top_p', top_p, 0.0, 1.0),
-        ('min_p', min_p, 0.0, 1.0))]
-    token = torch.empty(rows, dtype=torch.int64, device=x.device) if out is None else out
-    logp = torch.empty(rows, dtype=torch.float32, device=x.device) if return_log_probs else None
+    ops._need_cuda(logits, u, out)
+    x = logits if V == 1 or logits.stride(1) == 1 else logits.detach().contiguous()
+    dev = x.device
+    params = [_per_row('temperature', temperature, rows, dev), _per_row('top_k', top_k, rows, dev),
+              _per_row('top_p', top_p, rows, dev), _per_row('min_p', min_p, rows, dev)]
+    token = torch.empty(rows, dtype=torch.int64, device=dev) if out is None else out
+    logp = torch.empty(rows, dtype=torch.float32, device=dev) if return_log_probs else None
     if rows:
-        ops.sample(x, x.stride(0), rows, V, u.detach().contiguous(), token, token.stride(0), logp, *params)
+        ops.sample(x, x.stride(0), rows, V, u if u.is_contiguous() else u.contiguous(), token, token.stride(0), logp, *params)
     return (token, logp) if return_log_probs else token
