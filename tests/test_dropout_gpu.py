@@ -40,9 +40,7 @@ def test_forward_and_backward(dtype, n, p):
     assert torch.equal(dx, expect(dy, threshold(p), seed, offset))
 
 
-def test_more_elements_than_one_round_of_the_grid():
-    """The launch has at most 16384 workgroups of 256 threads with 8 elements each: the elements past 2^25 come in a second
-    round."""
+def test_many_elements_and_the_counter_running_over():
     from vqa_amd.dropout import dropout, threshold
     n = 2 ** 25 + 2 ** 14 + 5
     x = torch.ones(n, dtype=torch.bfloat16, device=dev())

@@ -34,6 +34,15 @@ __device__ __forceinline__ bool logp_live(const LogpRows& P, int64_t token) {
     return token >= 0 && token < P.V && token != P.ignore;
 }
 
+// Elements in front of a row's first 16-byte boundary.  Forward, the parts of a row start there and the first one takes these as
+// well: pieces that straddle cache lines cost a fifth of the bandwidth (8192 x 50001 bf16: 136 us, aligned 108).  Backward, with
+// two pieces a thread, finding the boundary costs more than it gives (253 us, aligned 267).
+template <int DT> __device__ __forceinline__ int logp_head(const typename Elem<DT>::type* row, int32_t V) {
+    constexpr int N = Elem<DT>::N, SIZE = 16 / N;
+    const int n = (N - (int)((uintptr_t)row % 16) / SIZE) % N;
+    return n < V ? n : V;
+}
+
 // m: maximum, at least the lowest float (so that differences of maxima are numbers); s, t: sums relative to it
 struct Mst { float m, s, t; };
 
@@ -81,7 +90,7 @@ __device__ __forceinline__ void logp_finish(const LogpRows& P, int64_t row, int6
 }
 
 // G threads a row: 8 to 64 of a wave, 256 / G rows a workgroup; or the whole workgroup (G = 256), for one part of a row.
-template <int DT, int G, bool ENT>
+template <int DT, int G, bool ENT, bool NT>
 __global__ __launch_bounds__(256) void logp_forward_kernel(LogpRows P, float* __restrict__ logp, float* __restrict__ entropy,
                                                            float4* __restrict__ stats, float4* __restrict__ partial) {
     typedef typename Elem<DT>::type T;
@@ -103,21 +112,26 @@ __global__ __launch_bounds__(256) void logp_forward_kernel(LogpRows P, float* __
             continue;
         }
         const T* x = logp_row<DT>(P, row);
-        const int64_t lo = part * P.chunk, hi = lo + P.chunk < P.V ? lo + P.chunk : P.V;
-        const int64_t nv = (hi - lo) / N;
+        const int head = logp_head<DT>(x, P.V);
+        const int64_t lo = head + part * P.chunk, hi = lo + P.chunk < P.V ? lo + P.chunk : P.V;
+        const int64_t nv = hi > lo ? (hi - lo) / N : 0;
         Mst a = {-FLT_MAX, 0.f, 0.f};
+        if (part == 0 && lane < head) {
+            const float f = elem_get<DT>(x + lane);
+            mst_add<1, ENT>(a, &f, P.c);
+        }
         int64_t v = lane;
         for (; v + (U - 1) * G < nv; v += U * G) {
             u32x4 r[U];
             float f[U * N];
 #pragma unroll
-            for (int k = 0; k < U; k++) r[k] = vec_load<DT>(x + lo + (v + k * G) * N);
+            for (int k = 0; k < U; k++) r[k] = vec_load_as<DT, NT>(x + lo + (v + k * G) * N);
 #pragma unroll
             for (int k = 0; k < U * N; k++) f[k] = vec_get<DT>(r[k / N], k % N);
             mst_add<U * N, ENT>(a, f, P.c);
         }
         for (; v < nv; v += G) {
-            const u32x4 r = vec_load<DT>(x + lo + v * N);
+            const u32x4 r = vec_load_as<DT, NT>(x + lo + v * N);
             float f[N];
 #pragma unroll
             for (int k = 0; k < N; k++) f[k] = vec_get<DT>(r, k);
@@ -159,7 +173,7 @@ __global__ __launch_bounds__(64) void logp_merge_kernel(LogpRows P, float* __res
 
 // dx_i = p_i (a + b (x_i - m)) (+ g / T at the token), p_i = 2^((x_i - m) c - log2 s);
 // a = -(g + h (H - log s)) / T, b = -h / T^2
-template <int DT, int G, bool ENT>
+template <int DT, int G, bool ENT, bool NT>
 __global__ __launch_bounds__(256) void logp_backward_kernel(LogpRows P, const float4* __restrict__ stats,
                                                             const float* __restrict__ gp, const float* __restrict__ hp,
                                                             typename Elem<DT>::type* __restrict__ dx) {
@@ -179,7 +193,7 @@ __global__ __launch_bounds__(256) void logp_backward_kernel(LogpRows P, const fl
         const float4 st = stats[row];
         if (!logp_live(P, token) || st.y == -INFINITY) {     // padding, or a row that nothing is left of
             const u32x4 zero = {0, 0, 0, 0};
-            for (int64_t v = lane; v < nv; v += G) vec_store<DT>(out + lo + v * N, zero);
+            for (int64_t v = lane; v < nv; v += G) vec_store_as<DT, NT>(out + lo + v * N, zero);
             for (int64_t i = lo + nv * N + lane; i < hi; i += G) elem_put<DT>(out + i, 0.f);
             continue;
         }
@@ -193,11 +207,11 @@ __global__ __launch_bounds__(256) void logp_backward_kernel(LogpRows P, const fl
         };
         for (int64_t v = lane; v < nv; v += G) {
             const int64_t i = lo + v * N;
-            const u32x4 r = vec_load<DT>(x + i);
+            const u32x4 r = vec_load_as<DT, NT>(x + i);
             float f[N];
 #pragma unroll
             for (int k = 0; k < N; k++) f[k] = grad(vec_get<DT>(r, k)) + (i + k == token ? gt : 0.f);
-            vec_store<DT>(out + i, vec_make<DT>(f));
+            vec_store_as<DT, NT>(out + i, vec_make<DT>(f));
         }
         for (int64_t i = lo + nv * N + lane; i < hi; i += G)
             elem_put<DT>(out + i, grad(elem_get<DT>(x + i)) + (i == token ? gt : 0.f));
@@ -246,17 +260,34 @@ static int logp_args(LogpRows& P, const char* who, const void* x, int64_t inner,
     return VQA_OK;
 }
 
+// Whether the logits are too many to stay in the last-level cache (256 MiB) from one pass to the next: then they are read,
+// and the gradient is written, past it (4096 x 131072 bf16: forward 162 -> 148 us, backward 312 -> 302; 2048 x 32768 fp16, which
+// stay: backward 36 -> 40).
+static bool logp_streams(const LogpRows& P, int dtype) {
+    return (double)P.rows * P.V * (dtype == VQA_F32 ? 4 : 2) > 256.0 * (1 << 20);
+}
+template <int DT, int G, bool NT>
+static void logp_forward_as(const LogpRows& P, dim3 grid, float* logp, float* entropy, float4* stats, float4* ws, hipStream_t s) {
+    if (entropy) hipLaunchKernelGGL((logp_forward_kernel<DT, G, true, NT>), grid, dim3(256), 0, s, P, logp, entropy, stats, ws);
+    else hipLaunchKernelGGL((logp_forward_kernel<DT, G, false, NT>), grid, dim3(256), 0, s, P, logp, entropy, stats, ws);
+}
 template <int DT, int G>
 static void logp_forward_launch(const LogpRows& P, dim3 grid, float* logp, float* entropy, float4* stats, float4* ws, hipStream_t s) {
-    if (entropy) hipLaunchKernelGGL((logp_forward_kernel<DT, G, true>), grid, dim3(256), 0, s, P, logp, entropy, stats, ws);
-    else hipLaunchKernelGGL((logp_forward_kernel<DT, G, false>), grid, dim3(256), 0, s, P, logp, entropy, stats, ws);
+    if (G == 256 && logp_streams(P, DT)) logp_forward_as<DT, G, G == 256>(P, grid, logp, entropy, stats, ws, s);
+    else logp_forward_as<DT, G, false>(P, grid, logp, entropy, stats, ws, s);
+}
+template <int DT, int G, bool NT>
+static void logp_backward_as(const LogpRows& P, dim3 grid, const float4* stats, const float* g, const float* h, void* dx,
+                             hipStream_t s) {
+    typedef typename Elem<DT>::type T;
+    if (h) hipLaunchKernelGGL((logp_backward_kernel<DT, G, true, NT>), grid, dim3(256), 0, s, P, stats, g, h, (T*)dx);
+    else hipLaunchKernelGGL((logp_backward_kernel<DT, G, false, NT>), grid, dim3(256), 0, s, P, stats, g, h, (T*)dx);
 }
 template <int DT, int G>
 static void logp_backward_launch(const LogpRows& P, dim3 grid, const float4* stats, const float* g, const float* h, void* dx,
                                  hipStream_t s) {
-    typedef typename Elem<DT>::type T;
-    if (h) hipLaunchKernelGGL((logp_backward_kernel<DT, G, true>), grid, dim3(256), 0, s, P, stats, g, h, (T*)dx);
-    else hipLaunchKernelGGL((logp_backward_kernel<DT, G, false>), grid, dim3(256), 0, s, P, stats, g, h, (T*)dx);
+    if (G == 256 && logp_streams(P, DT)) logp_backward_as<DT, G, G == 256>(P, grid, stats, g, h, dx, s);
+    else logp_backward_as<DT, G, false>(P, grid, stats, g, h, dx, s);
 }
 #define LOGP_GROUPS(FN, DT, ...)                             \
     switch (G) {                                             \
@@ -319,8 +350,8 @@ extern "C" int vqa_token_logp_backward(const void* x, int64_t inner, int64_t ld_
     }
     if (rows == 0) return VQA_OK;
     const int G = logp_group(V, dtype);
-    // a workgroup's part of a long row: four 16-byte pieces a thread
-    P.chunk = G == 256 ? 4 * 256 * (dtype == VQA_F32 ? 4 : 8) : V;
+    // a workgroup's part of a long row: two 16-byte pieces a thread (with four, 4096 x 131072 bf16 took 340 us, with two 312)
+    P.chunk = G == 256 ? 2 * 256 * (dtype == VQA_F32 ? 4 : 8) : V;
     P.parts = (int32_t)((V + P.chunk - 1) / P.chunk);
     const dim3 grid = logp_grid(P, G);
     LOGP_DISPATCH(logp_backward_launch, P, grid, (const float4*)stats, g, h, dx, (hipStream_t)stream)

@@ -42,6 +42,15 @@ template <int DT> __device__ __forceinline__ void elem_put(typename Elem<DT>::ty
 template <int DT> __device__ __forceinline__ u32x4 vec_load(const typename Elem<DT>::type* p) {
     return *(const u32x4u*)p;
 }
+// NT: past the last-level cache, for what will not be there any more when it is read again
+template <int DT, bool NT> __device__ __forceinline__ u32x4 vec_load_as(const typename Elem<DT>::type* p) {
+    if constexpr (NT) return __builtin_nontemporal_load((const u32x4u*)p);
+    else return *(const u32x4u*)p;
+}
+template <int DT, bool NT> __device__ __forceinline__ void vec_store_as(typename Elem<DT>::type* p, u32x4 v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, (u32x4u*)p);
+    else *(u32x4u*)p = v;
+}
 template <int DT> __device__ __forceinline__ void vec_store(typename Elem<DT>::type* p, u32x4 v) { *(u32x4u*)p = v; }
 // element i of a 16-byte piece as a float
 template <int DT> __device__ __forceinline__ float vec_get(u32x4 v, int i) {
