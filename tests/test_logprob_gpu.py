@@ -236,3 +236,25 @@ def test_a_change_between_forward_and_backward_is_refused():
         x.add_(1)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         lp.sum().backward()
+
+
+def test_saved_tensor_hooks_may_move_what_backward_reads():
+    """Offloading (torch.autograd.graph.save_on_cpu) hands backward other tensors than forward saved, with other strides."""
+    from vqa_amd.dropout import dropout
+    from vqa_amd.loss import token_log_probs
+    base = logits((3, 6, 101), 2, torch.bfloat16)
+    tk = tokens_for((3, 5), 101, 1).to(dev())
+    state = torch.tensor([3, 4], dtype=torch.int64, device=dev())
+    got = []
+    for hooks in (None, torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t)):
+        leaf = base.clone().requires_grad_(True)
+        if hooks is None:
+            lp = token_log_probs(dropout(leaf, 0.2, state)[:, :-1], tk)
+        else:
+            with hooks:
+                lp = token_log_probs(dropout(leaf, 0.2, state)[:, :-1], tk)
+        scratch = [torch.full((3, 6, 101), 7.0, dtype=torch.bfloat16, device=dev()) for _ in range(4)]     # in freed memory
+        got.append((lp.detach(), torch.autograd.grad(lp.sum(), leaf)[0]))
+        del scratch
+    for other in got[1:]:
+        assert torch.equal(got[0][0], other[0]) and torch.equal(got[0][1], other[1])

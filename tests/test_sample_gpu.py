@@ -244,7 +244,7 @@ def test_lists_of_every_length(dtype, V):
     """Around the capacity of the list of candidates (2048): top-k beyond it, many equal logits at the cut, a bin edge that
     falls on 0 (symmetric rows), rows far from 0, tiny and huge spreads."""
     g = torch.Generator().manual_seed(V)
-    x = torch.randn(10, V, generator=g) * 2
+    x = torch.randn(11, V, generator=g) * 2
     x[1] = torch.linspace(-10, 10, V)
     x[2] = torch.randint(0, 3, (V,), generator=g).float()
     x[3] = torch.randint(0, 40, (V,), generator=g) * 0.25
@@ -254,8 +254,9 @@ def test_lists_of_every_length(dtype, V):
     x[7, : V // 2] = 5.0
     x[8] = torch.linspace(-1e-30, 1e-30, V)
     x[9, 0] = -1e30
+    x[10] = torch.arange(V) * 1e-43 - 3e-41          # subnormal numbers (zeros in fp16)
     x = x.to(dtype).to(dev())
     for params in (dict(), dict(top_k=2000), dict(top_k=2048), dict(top_k=2049, top_p=0.9), dict(top_p=0.7),
                    dict(top_p=0.999, min_p=0.01), dict(min_p=1.0), dict(temperature=0.01, top_p=0.9), dict(temperature=100.0)):
         for u in (0.0, 0.4, 0.93, 1 - 2.0 ** -24):
-            check(x, torch.full((10,), u), **params)
+            check(x, torch.full((11,), u), **params)

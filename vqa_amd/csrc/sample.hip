@@ -871,7 +871,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     }
     __syncthreads();
     const float e0 = uniform(L.edge[0]), e1 = uniform(L.edge[1]), e2 = uniform(L.edge[2]), e3 = uniform(L.edge[3]);
-    H.template each<2>([&](float f, int i) {
+    H.template each<4>([&](float f, int i) {
         if (((f >= e0) & (f < e1)) | ((f >= e2) & (f < e3))) {
             const uint32_t at = atomicAdd(&L.n, 1u);
             if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), first_index + i);
@@ -893,7 +893,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
         if ((int)L.pick != P.parts - 1) return;
         n = (int)__hip_atomic_load(&Q->n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if (n > LIST) {
+    if (n > LIST || n == 0) {
         radix_row<DT, BT, RB>((LDS_AS void*)&shared, P, row);
         return;
     }

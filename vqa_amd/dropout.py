@@ -33,9 +33,9 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, thr, seed, offset, state):
         x = x.contiguous()
         y = torch.empty_like(x)
-        ctx.call = ops.dropout(x, y, thr, seed, offset, state)
-        if state is not None:
-            ctx.save_for_backward(state)      # (changed before backward, it would give another mask: autograd refuses that)
+        ops.dropout(x, y, thr, seed, offset, state)
+        ctx.args = thr, seed, offset
+        ctx.save_for_backward(state)          # (changed before backward, it would give another mask: autograd refuses that)
         return y
 
     @staticmethod
@@ -45,10 +45,10 @@ class _Dropout(torch.autograd.Function):
 
 def _dropout_grad(ctx, dy):
     # (as little as can be: what runs in autograd's thread takes three times as long as in the caller's)
-    ctx.saved_tensors
+    (state,) = ctx.saved_tensors
     dy = dy.contiguous()
     dx = torch.empty_like(dy)
-    ops.dropout_again(dy, dx, ctx.call)
+    ops.dropout(dy, dx, *ctx.args, state)
     return dx, None, None, None, None
 
 

@@ -59,10 +59,11 @@ class _TokenLogProbs(torch.autograd.Function):
         lp = torch.empty(tokens.shape, dtype=torch.float32, device=x.device)
         ent = torch.empty_like(lp) if want_entropy else None
         stats = torch.empty(layout[0], 4, dtype=torch.float32, device=x.device)
-        ctx.call = ops.token_logp(x, layout, tk, lp, ent, stats, x.size(-1), temperature, ignore) if layout[0] else None
+        if layout[0]:
+            ops.token_logp(x, layout, tk, lp, ent, stats, x.size(-1), temperature, ignore)
         # (the caller's own tensor where it was read in place: autograd then notices a change before backward)
         ctx.save_for_backward(x, tk, stats)
-        ctx.like = logits.shape, x.dtype, x.device
+        ctx.args = x.data_ptr(), layout, logits.shape, temperature, ignore
         return (lp, ent) if want_entropy else lp
 
     @staticmethod
@@ -72,13 +73,16 @@ class _TokenLogProbs(torch.autograd.Function):
 
 def _log_probs_grad(ctx, g, h):
     # (as little as can be: what runs in autograd's thread takes three times as long as in the caller's)
-    ctx.saved_tensors
     if g is None and h is None:
         return None, None, None, None, None
-    shape, dtype, device = ctx.like
-    dx = torch.empty(shape, dtype=dtype, device=device)
-    if ctx.call is not None:
-        ops.token_logp_backward(ctx.call, g if g is None else g.contiguous(), h if h is None else h.contiguous(), dx)
+    x, tk, stats = ctx.saved_tensors
+    ptr, layout, shape, temperature, ignore = ctx.args
+    if x.data_ptr() != ptr:                   # (a saved-tensor hook has put it elsewhere, with strides of its own)
+        x, *layout = ops.row_layout(x)
+    dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if layout[0]:
+        ops.token_logp_backward(x, layout, tk.contiguous(), stats.contiguous(), g if g is None else g.contiguous(),
+                                h if h is None else h.contiguous(), dx, shape[-1], temperature, ignore)
     return dx, None, None, None, None
 
 

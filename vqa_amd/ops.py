@@ -392,7 +392,7 @@ def row_layout(x):
 
 def token_logp(x, layout, tokens, logp, entropy, stats, V, temperature, ignore):
     """logp, entropy (or None) fp32 [rows], stats fp32 [rows, 4] of int64 tokens [rows] under softmax(x / temperature);
-    layout: (rows, inner, ld_inner, ld_outer) of x.  Returns what token_logp_backward() needs."""
+    layout: (rows, inner, ld_inner, ld_outer) of x"""
     rows, inner, ld_inner, ld_outer = layout
     _same_device(x, tokens, logp, entropy, stats)
     assert tokens.dtype == torch.int64 and tokens.is_contiguous() and tokens.numel() == rows
@@ -401,31 +401,25 @@ def token_logp(x, layout, tokens, logp, entropy, stats, V, temperature, ignore):
     lib, dt = _lib.load(), ROW_DTYPES[x.dtype]
     need = lib.vqa_token_logp_workspace(rows, V, dt)
     ws = torch.empty(need, dtype=torch.float32, device=x.device) if need else None
-    where, what = (_addr(x), inner, ld_inner, ld_outer, _addr(tokens)), (rows, V, dt, temperature, ignore)
-    _call_on(x, lib.vqa_token_logp, *where, _addr(logp), _addr(entropy), _addr(stats), _addr(ws), *what)
-    return where + (_addr(stats),), what
+    _call_on(x, lib.vqa_token_logp, _addr(x), inner, ld_inner, ld_outer, _addr(tokens), _addr(logp), _addr(entropy), _addr(stats),
+             _addr(ws), rows, V, dt, temperature, ignore)
 
 
-def token_logp_backward(call, g, h, dx):
-    """dx [rows, V] dense, of x's type, from what token_logp() returned (its tensors still alive and unchanged); g, h: fp32
-    [rows], contiguous, or None"""
-    _call_on(dx, _lib.load().vqa_token_logp_backward, *call[0], _addr(g), _addr(h), dx.data_ptr(), *call[1])
+def token_logp_backward(x, layout, tokens, stats, g, h, dx, V, temperature, ignore):
+    """dx [rows, V] dense, of x's type; stats as token_logp() wrote them; g, h: fp32 [rows], contiguous, or None.  (Shapes and
+    types are the caller's care here: this runs in autograd's thread.)"""
+    rows, inner, ld_inner, ld_outer = layout
+    _call_on(x, _lib.load().vqa_token_logp_backward, x.data_ptr(), inner, ld_inner, ld_outer, tokens.data_ptr(), stats.data_ptr(),
+             _addr(g), _addr(h), dx.data_ptr(), rows, V, ROW_DTYPES[x.dtype], temperature, ignore)
 
 
 def dropout(x, y, threshold, seed, offset, state=None):
-    """y = x with the elements dropped whose random bits are below threshold (vqa_dropout); y may be x.  Returns what
-    dropout_again() needs for the same mask."""
+    """y = x with the elements dropped whose random bits are below threshold (vqa_dropout); y may be x"""
     _same_device(x, y, state)
     assert x.dtype == y.dtype and x.is_contiguous() and y.is_contiguous() and y.numel() >= x.numel()
     assert state is None or (state.dtype == torch.int64 and state.is_contiguous() and state.numel() == 2)
-    call = (x.numel(), ROW_DTYPES[x.dtype], threshold, seed & 2 ** 64 - 1, offset & 2 ** 64 - 1, _addr(state))
-    _call_on(x, _lib.load().vqa_dropout, _addr(x), _addr(y), *call)
-    return call
-
-
-def dropout_again(x, y, call):
-    """The mask of an earlier dropout() on another pair of tensors of its size and type."""
-    _call_on(x, _lib.load().vqa_dropout, x.data_ptr(), y.data_ptr(), *call)
+    _call_on(x, _lib.load().vqa_dropout, x.data_ptr(), y.data_ptr(), x.numel(), ROW_DTYPES[x.dtype], threshold, seed & 2 ** 64 - 1,
+             offset & 2 ** 64 - 1, _addr(state))
 
 
 def slot_sum_mask(arena, blob, off_offsets, off_src, off_dst, off_mask, n_dst, slot_elems):
