@@ -93,7 +93,7 @@ def test_filters(dtype, rows, V, params):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [44, 700, 9000, 36000])
+@pytest.mark.parametrize('V', [44, 700, 9000, 83000])
 def test_every_row_its_own_parameters(dtype, V):
     rows = 48
     g = torch.Generator().manual_seed(V)
@@ -116,7 +116,7 @@ def test_parameters_outside_their_range_in_a_tensor(V):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [44, 64, 300, 9001, 40009])
+@pytest.mark.parametrize('V', [44, 64, 300, 9001, 50009])
 def test_masks_infinities_and_nan(dtype, V):
     x = logits(12, V, V, dtype)
     x[0, :] = -math.inf
@@ -137,7 +137,7 @@ def test_masks_infinities_and_nan(dtype, V):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [50, 1000, 10000, 33000])
+@pytest.mark.parametrize('V', [50, 1000, 10000, 40000])
 def test_ties_go_by_index(dtype, V):
     """Constant rows and rows of two values: the cut of top-k and top-p falls among equals."""
     x = torch.zeros(4, V, dtype=dtype, device=dev())
@@ -188,7 +188,7 @@ def test_more_rows_than_workgroups():
     check(x[:64], u[:64].cpu())
 
 
-@pytest.mark.parametrize('V', [2000, 20000, 33333])
+@pytest.mark.parametrize('V', [2000, 20000, 100003])
 def test_the_same_row_in_batches_of_every_size(V):
     """How many rows a call has decides how a row is split and by how many threads it is done: the answers agree."""
     from vqa_amd.sampling import sample
@@ -196,7 +196,7 @@ def test_the_same_row_in_batches_of_every_size(V):
     u = uniform(300, V).to(dev())
     for params in (dict(top_p=0.9), dict(top_k=30), dict(temperature=0.5)):
         want = sample(x, u, return_log_probs=True, **params)
-        for n in (1, 60, 129, 256):
+        for n in (1, 64, 65, 256):
             got = sample(x[:n], u[:n], return_log_probs=True, **params)
             assert torch.equal(got[0], want[0][:n])
             assert ((got[1] - want[1][:n]).abs() <= want[1][:n].abs() * 2.0 ** -23).all()
@@ -204,7 +204,7 @@ def test_the_same_row_in_batches_of_every_size(V):
 
 def test_another_stream_and_a_captured_graph():
     from vqa_amd.sampling import sample
-    for V in (44, 5000, 20000, 40000):
+    for V in (44, 5000, 20000, 70000):
         x = logits(6, V, V, torch.float32)
         u = uniform(6, V).to(dev())
         want = sample(x, u, top_p=0.8, return_log_probs=True)

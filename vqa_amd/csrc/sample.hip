@@ -906,10 +906,11 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     finish_list<DT, BT, LIST>(L, swapped, P, row, r, W, n, by_count ? nullptr : B.front, S, total);
 }
 
-// Workgroups of a row.  Half of the device's 256 units are idle with 128 rows or fewer; a part keeps 8192 logits, below
-// which the four launches cost more than they save.
+// Workgroups of a row.  A split row pays for three launches and for a scan of its bins in each workgroup of the last: worth it
+// from 32768 logits on for a single row, from 98304 for 64 of them (bf16, top-p 0.9, split against whole: 1 x 50001 23 / 27 us,
+// 1 x 131072 26 / 51, 8 x 65536 32 / 36, 64 x 65536 42 / 36, 64 x 131072 52 / 56), not with more rows (128 x 131072 63 / 59).
 static int sample_parts(int64_t rows, int32_t V) {
-    if (rows <= 0 || rows > 128 || V < 4 * 8192) return 1;
+    if (rows <= 0 || rows > 64 || V < 32768 + 1024 * rows) return 1;
     const int64_t by_rows = 256 / rows, by_size = V / 8192;
     const int64_t parts = by_rows < by_size ? by_rows : by_size;
     return (int)(parts < SPLIT_PARTS ? parts : SPLIT_PARTS);
