@@ -260,3 +260,32 @@ def test_lists_of_every_length(dtype, V):
                    dict(top_p=0.999, min_p=0.01), dict(min_p=1.0), dict(temperature=0.01, top_p=0.9), dict(temperature=100.0)):
         for u in (0.0, 0.4, 0.93, 1 - 2.0 ** -24):
             check(x, torch.full((11,), u), **params)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('V', [16384, 20011])
+def test_rows_whose_parts_differ(dtype, V):
+    """Long rows are laid out by what a sixteenth of them shows: rows that rise or fall, whose front is masked, constant or
+    narrow, with a few or many tokens above and below everything in front of them."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(14, V, generator=g) * 2
+    end = slice(V - 2500, V)
+    x[0] = torch.linspace(-9, 9, V)
+    x[1] = torch.linspace(9, -9, V)
+    x[2, : V - 3000] = -math.inf
+    x[3, : V - 3000] = 1.0
+    x[4, V - 40: V - 37] = torch.tensor([14.0, 15.0, 16.0])
+    x[5, V - 40: V - 30] = -16.0
+    x[6, V - 3] = math.inf
+    x[7, end] = math.nan
+    x[8, end] = 11.0
+    x[9, V - 5] = 60.0
+    x[10, : V - 3000] *= 1e-3
+    x[11, end] = -12.0
+    x[12, V - 700: V - 100] = 10 + torch.rand(600, generator=g) * 3
+    x[13, V - 30: V - 10] = -3000.0
+    x = x.to(dtype).to(dev())
+    for params in (dict(), dict(top_k=1), dict(top_k=30), dict(top_k=1500), dict(top_p=0.9), dict(top_p=0.2), dict(top_p=0.9999),
+                   dict(temperature=0.05, top_p=0.9), dict(temperature=20.0), dict(min_p=0.01), dict(temperature=0.0)):
+        for u in (0.0, 0.3, 0.8, 1 - 2.0 ** -24):
+            check(x, torch.full((14,), u), **params)

@@ -421,14 +421,19 @@ template <int DT, int BT, int RB> __device__ __attribute__((noinline)) void radi
 // draw are looked up in it.  Rows whose list would be too long - many equal logits - go to the radix search.
 #define LIST_ALL 128
 #define WINDOW 40.0
+#define GUESS_FROM 16384
 
 typedef Keys<VQA_F32> FKeys;       // the list's keys: of the logits as fp32, whatever their type
 
 // Steps of x below the maximum: bin b holds the x with floor(at(x)) = b, at(x) = (max - x) scale + 1/2.
 struct Steps {
     double max, scale;             // (the difference first: max * scale may dwarf the 1/2)
+    float hi, lo;                  // what the bins hold: lo <= x <= hi
+    int bins;
     __device__ __forceinline__ double at(float x) const { return fma(max - (double)x, scale, 0.5); }
     __device__ __forceinline__ uint32_t bin(float x) const { return (uint32_t)at(x); }
+    // bin, or a place of its own for what lies below and above the bins
+    __device__ __forceinline__ uint32_t slot(float x) const { return x > hi ? bins + 1 : x < lo ? bins : bin(x); }
 };
 
 // One wave: the smallest float in [bottom, top] that `in` holds for; it holds for `top`, and for every float above one that
@@ -459,12 +464,13 @@ template <int CAP> struct ListShared {
         unsigned long long other[CAP];
     };
     double part[16], total, behind;      // total: the kept weight; behind: the weight up to the nucleus's last bin
+    unsigned long long above, below;     // weight, or number, of the tokens outside the bins
     float max[16], min[16], edge[4], lo;
-    uint32_t n, last, pick, bin_end, bin_lo, bin_hi;
+    uint32_t n, top, last, pick, bin_end, bin_lo, bin_hi;
 };
 template <int BINS> union BinShared {
     unsigned long long mass[BINS];       // weights, or the numbers of tokens
-    double front[BINS];                  // the weight in front of each bin
+    double front[BINS + 2];              // the weight in front of each bin, of what is below the bins, of what is above
 };
 
 // exclusive sums of v over the workgroup's threads, in thread order
@@ -554,7 +560,7 @@ __device__ __forceinline__ void finish_list(ListShared<CAP>& L, bool swapped, co
     }
     if (tid == 0) L.last = L.pick = 0;
     const double before = scan_threads<BT>(L.part, sum, listed);
-    auto bin_of = [&](int i) { return S.bin((float)FKeys::value((uint32_t)(list[i] >> 32))); };
+    auto bin_of = [&](int i) { return S.slot((float)FKeys::value((uint32_t)(list[i] >> 32))); };
     if (front) {                                             // front[b] becomes what is in front of the bin beyond the list
         double g = before;
         for (int i = i0; i < i1; i++) {
@@ -655,6 +661,15 @@ template <int DT, int BT> struct RowPass {
     const T* x;
     int V, nv;
     __device__ __forceinline__ RowPass(const T* x_, int V_) : x(x_), V(V_), nv(V_ / N) {}
+    // calls f(x) with a sixteenth of the logits or more, in stretches all over the row
+    template <typename F> __device__ __forceinline__ void some(F f) const {
+#pragma unroll 4
+        for (int v = threadIdx.x; v < nv; v += 16 * BT) {
+            const u32x4 r = vec_load<DT>(x + (int64_t)v * N);
+#pragma unroll
+            for (int q = 0; q < N; q++) f(vec_get<DT>(r, q), 0);
+        }
+    }
     // calls f(x, index) with every logit as a float; U pieces of 16 bytes on their way at a time
     template <int U, typename F> __device__ __forceinline__ void each(F f) const {
         int v = threadIdx.x;
@@ -683,12 +698,12 @@ template <int DT, int BT> struct RowPass {
 
 template <int BT, int BINS> struct BinScan {
     static constexpr int PER = BINS / BT;
-    // front[b]: the sum of v over the bins before b; v: the thread's bins, read from where front goes
-    static __device__ __forceinline__ double scan(BinShared<BINS>& B, double* part, const double (&v)[PER]) {
+    // front[b]: `above` and the sum of v over the bins before b; v: the thread's bins, read from where front goes
+    static __device__ __forceinline__ double scan(BinShared<BINS>& B, double* part, const double (&v)[PER], double above) {
         double sum = 0.0, total;
 #pragma unroll
         for (int k = 0; k < PER; k++) sum += v[k];
-        double g = scan_threads<BT>(part, sum, total);
+        double g = above + scan_threads<BT>(part, sum, total);
 #pragma unroll
         for (int k = 0; k < PER; k++) {
             B.front[threadIdx.x * PER + k] = g;
@@ -733,92 +748,131 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     SplitRow* const Q = P.split + (SPLIT ? row : 0);
     const int first_index = part * P.part_size;
     const RowPass<DT, BT> H((const T*)P.x + row * P.ld + first_index, SPLIT ? ::min(P.part_size, P.V - first_index) : P.V);
-    float max = -INFINITY, min = INFINITY;
-    if (PHASE == WHOLE || PHASE == HISTOGRAM)
-        for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
-    if (tid == 0) L.n = L.bin_end = L.bin_lo = L.bin_hi = 0;
-    if (PHASE == WHOLE || PHASE == MAXIMUM) {
-        H.template each<4>([&](float f, int) {
-            max = fmaxf(max, f);                             // (a NaN is passed over)
-            min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
-        });
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            max = fmaxf(max, __shfl_xor(max, d));
-            min = fminf(min, __shfl_xor(min, d));
-        }
-        if ((tid & 63) == 0) {
-            L.max[wave] = max;
-            L.min[wave] = min;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < BT / 64; w++) {
-            max = fmaxf(max, L.max[w]);
-            min = fminf(min, L.min[w]);
-        }
-    } else {
-        __syncthreads();
-        for (int q = 0; q < P.parts; q++) {
-            max = fmaxf(max, Q->max[q]);
-            min = fminf(min, Q->min[q]);
-        }
-    }
-    if (PHASE == MAXIMUM) {
-        for (int b = part * BT + tid; b < BINS; b += P.parts * BT) Q->hist[b] = 0;
-        if (tid == 0) {
-            Q->max[part] = max;
-            Q->min[part] = min;
-            if (part == 0) Q->n = Q->done = 0;
-        }
-        return;
-    }
     const RowParams r = row_params(P, row);
-    max = uniform(max);
-    min = uniform(min);
-    if (max == -INFINITY) {
-        if (tid == 0 && part == 0) sample_put<DT>(P, row, -1, -INFINITY);
-        return;
-    }
-    if (max == INFINITY || max == min) {
-        if (PHASE == WHOLE || (PHASE == COLLECT && part == 0)) radix_row<DT, BT, RB>((LDS_AS void*)&shared, P, row);
-        return;
-    }
-    const Weights<VQA_F32> W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
-    const double range = uniform(fmin((double)max - (double)min, WINDOW * r.t));
-    const Steps S = {W.max, uniform((BINS - 1) / range)};
-    float lo = min;
-    if (r.min_p > 0.0 || (double)max - (double)min > range) {
-        if (wave == 0) {
-            const float f = first_float(min, max, [&](float f) {
-                return (double)max - (double)f <= range && ((double)f - W.max) * W.inv_t >= W.min_z;
-            });
-            if (tid == 0) L.lo = f;
-        }
-        __syncthreads();
-        lo = uniform(L.lo);
-    }
     const bool by_count = r.k > 0 && r.k < P.V;
-    const double d = uniform(W.inv_t / S.scale);         // a step of the bins in z
-    if (PHASE == WHOLE || PHASE == HISTOGRAM) {
-        if (by_count) {
-            H.template each<2>([&](float f, int) {
-                if (f >= lo) atomicAdd((uint32_t*)&B.mass[S.bin(f)], 1u);
-            });
-        } else {
-            // e^(-(f - 1/2) d) for 0 <= f < 1: the series around 1/2, in powers of f (and `magic` on top)
-            const double c1 = -d, c2 = d * d * 0.5, c3 = d * d * d * (-1.0 / 6.0), c4 = d * d * d * d * (1.0 / 24.0);
-            const double a3 = uniform(c3 - 2.0 * c4), a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4);
-            const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4);
-            const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 + W.magic);
-            const long long magic = __double_as_longlong(W.magic);
-            H.template each<2>([&](float f, int) {
-                if (!(f >= lo)) return;
-                const double a = S.at(f), e = __builtin_amdgcn_fract(a);
-                const double p = fma(e, fma(e, fma(e, fma(e, c4, a3), a2), a1), a0);
-                atomicAdd(&B.mass[(uint32_t)a], (unsigned long long)(__double_as_longlong(p) - magic));
-            });
+    // The maximum of a whole row costs a pass over memory in which little is computed, and the histogram is bound by
+    // arithmetic.  Without min-p (which needs the true maximum) long rows take both passes as one: the bins lie between the
+    // largest and the smallest logit of a sixteenth of the row, and the few tokens outside go on the list at once.  If they
+    // are not few, it starts again with the whole row's.
+    bool guess = PHASE == WHOLE && P.V >= GUESS_FROM && !(r.min_p > 0.0);
+    float max, min;
+    Weights<VQA_F32> W;
+    Steps S;
+    double d;                                                // a step of the bins in z
+    for (;; guess = false) {
+        max = -INFINITY, min = INFINITY;
+        if (PHASE == WHOLE || PHASE == HISTOGRAM)
+            for (int b = tid; b < BINS; b += BT) B.mass[b] = 0;
+        if (tid == 0) {
+            L.n = L.top = L.bin_end = L.bin_lo = L.bin_hi = 0;
+            L.above = L.below = 0;
         }
+        if (PHASE == WHOLE || PHASE == MAXIMUM) {
+            auto widen = [&](float f, int) {
+                max = fmaxf(max, f);                         // (a NaN is passed over)
+                min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
+            };
+            if (guess) H.some(widen);
+            else H.template each<4>(widen);
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) {
+                max = fmaxf(max, __shfl_xor(max, d));
+                min = fminf(min, __shfl_xor(min, d));
+            }
+            if ((tid & 63) == 0) {
+                L.max[wave] = max;
+                L.min[wave] = min;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < BT / 64; w++) {
+                max = fmaxf(max, L.max[w]);
+                min = fminf(min, L.min[w]);
+            }
+        } else {
+            __syncthreads();
+            for (int q = 0; q < P.parts; q++) {
+                max = fmaxf(max, Q->max[q]);
+                min = fminf(min, Q->min[q]);
+            }
+        }
+        if (PHASE == MAXIMUM) {
+            for (int b = part * BT + tid; b < BINS; b += P.parts * BT) Q->hist[b] = 0;
+            if (tid == 0) {
+                Q->max[part] = max;
+                Q->min[part] = min;
+                if (part == 0) Q->n = Q->done = 0;
+            }
+            return;
+        }
+        max = uniform(max);
+        min = uniform(min);
+        if (max == -INFINITY || max == INFINITY || max == min) {
+            if (guess) {
+                __syncthreads();                             // (L.max is written again)
+                continue;
+            }
+            if (max == -INFINITY) {
+                if (tid == 0 && part == 0) sample_put<DT>(P, row, -1, -INFINITY);
+            } else if (PHASE == WHOLE || (PHASE == COLLECT && part == 0)) {
+                radix_row<DT, BT, RB>((LDS_AS void*)&shared, P, row);
+            }
+            return;
+        }
+        W = row_weights<VQA_F32>(r, FKeys::of(__float_as_uint(max)), P.shift);
+        const bool cut = (double)max - (double)min > WINDOW * r.t;
+        const double range = uniform(cut ? WINDOW * r.t : (double)max - (double)min);
+        S.max = W.max;
+        S.scale = uniform((BINS - 1) / range);
+        S.hi = max;
+        S.lo = min;
+        S.bins = BINS;
+        if (r.min_p > 0.0 || cut) {
+            if (wave == 0) {
+                const float f = first_float(min, max, [&](float f) {
+                    return (double)max - (double)f <= range && ((double)f - W.max) * W.inv_t >= W.min_z;
+                });
+                if (tid == 0) L.lo = f;
+            }
+            __syncthreads();
+            S.lo = uniform(L.lo);
+        }
+        d = uniform(W.inv_t / S.scale);
+        if (PHASE == WHOLE || PHASE == HISTOGRAM) {
+            const float lo = S.lo;
+            // (what is further down than WINDOW weighs nothing)
+            const float least = guess && !cut ? uniform(fmaxf((float)((double)max - WINDOW * r.t), -FLT_MAX)) : lo;
+            auto outside = [&](float f, int i) {
+                if ((f > max) | ((f < lo) & (f >= least))) {
+                    const uint32_t at = atomicAdd(&L.n, 1u);
+                    if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), i);
+                }
+            };
+            if (by_count) {
+                H.template each<2>([&](float f, int i) {
+                    if ((f >= lo) & (f <= max)) atomicAdd((uint32_t*)&B.mass[S.bin(f)], 1u);
+                    else if (PHASE == WHOLE) outside(f, i);
+                });
+            } else {
+                // e^(-(f - 1/2) d) for 0 <= f < 1: the series around 1/2, in powers of f (and `magic` on top)
+                const double c1 = -d, c2 = d * d * 0.5, c3 = d * d * d * (-1.0 / 6.0), c4 = d * d * d * d * (1.0 / 24.0);
+                const double a3 = uniform(c3 - 2.0 * c4), a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4);
+                const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4);
+                const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 + W.magic);
+                const long long magic = __double_as_longlong(W.magic);
+                H.template each<2>([&](float f, int i) {
+                    if ((f >= lo) & (f <= max)) {
+                        const double a = S.at(f), e = __builtin_amdgcn_fract(a);
+                        const double p = fma(e, fma(e, fma(e, fma(e, c4, a3), a2), a1), a0);
+                        atomicAdd(&B.mass[(uint32_t)a], (unsigned long long)(__double_as_longlong(p) - magic));
+                    } else if (PHASE == WHOLE) {
+                        outside(f, i);
+                    }
+                });
+            }
+            __syncthreads();
+        }
+        if (!guess || L.n <= LIST / 2) break;
         __syncthreads();
     }
     if (PHASE == HISTOGRAM) {
@@ -826,10 +880,31 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
             if (B.mass[b]) atomicAdd(&Q->hist[b], B.mass[b]);
         return;
     }
+    double above = 0.0, below = 0.0, bins_top = 1.0;         // outside the bins; the weight of the bins' largest logit
+    if (guess && L.n > 0) {
+        const uint32_t guessed = W.top;
+        for (uint32_t i = tid; i < L.n; i += BT) atomicMax(&L.top, (uint32_t)(L.list[i] >> 32));
+        __syncthreads();
+        const uint32_t top = ::max(guessed, (uint32_t)__builtin_amdgcn_readfirstlane(L.top));
+        if (top == FKeys::TOP) {
+            radix_row<DT, BT, RB>((LDS_AS void*)&shared, P, row);
+            return;
+        }
+        W.top = top;
+        W.max = uniform(FKeys::value(top));
+        bins_top = exp(W.z(guessed));
+        for (uint32_t i = tid; i < L.n; i += BT) {
+            const uint32_t key = (uint32_t)(L.list[i] >> 32);
+            atomicAdd(key > guessed ? &L.above : &L.below, by_count ? 1ull : (unsigned long long)W.of(key));
+        }
+        __syncthreads();
+        above = by_count ? (double)L.above : ldexp((double)L.above, -P.shift);
+        below = by_count ? (double)L.below : ldexp((double)L.below, -P.shift);
+    }
     // the weight, or with top-k the number, of the tokens in each bin
     double v[PER];
     {
-        double weight = by_count ? 1.0 : ldexp(exp(-d * (tid * PER)), -P.shift);     // 2^-s e^(-b d) for the thread's first bin
+        double weight = by_count ? 1.0 : ldexp(bins_top * exp(-d * (tid * PER)), -P.shift);      // 2^-s e^(z of the thread's first bin)
         const double step = by_count ? 1.0 : exp(-d);
 #pragma unroll
         for (int q = 0; q < PER; q++) {
@@ -837,7 +912,11 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
             weight *= step;
         }
     }
-    const double total = BinScan<BT, BINS>::scan(B, L.part, v);
+    const double binned = above + BinScan<BT, BINS>::scan(B, L.part, v, above), total = binned + below;
+    if (tid == 0) {
+        B.front[BINS] = binned;
+        B.front[BINS + 1] = 0.0;
+    }
     if (by_count) {
         BinScan<BT, BINS>::last_bin(B, v, &L.bin_hi, (double)r.k, false);        // (or the last bin, where fewer tokens count)
     } else if (r.nucleus) {
@@ -848,7 +927,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
 #pragma unroll
             for (int q = 0; q < PER; q++)
                 if (q <= (int)L.bin_end % PER) g += v[q];
-            L.behind = g;
+            L.behind = r.top_p * total > binned ? total : g;
         }
         __syncthreads();
         BinScan<BT, BINS>::last_bin(B, v, &L.bin_lo, r.u * B.front[L.bin_end], true);
@@ -864,8 +943,9 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
         const uint32_t last = by_count ? L.bin_hi : wave >= 2 ? end : r.nucleus ? ::min(L.bin_hi, end) : first;
         float e = INFINITY;
         if (wave < 2 || (r.nucleus && !by_count)) {
-            if (!(wave & 1)) e = first_float(lo, max, [&](float f) { return S.bin(f) <= last; });
-            else if (first > 0) e = first_float(lo, max, [&](float f) { return S.bin(f) < first; });
+            if (!(wave & 1)) e = first_float(S.lo, max, [&](float f) { return S.bin(f) <= last; });
+            else if (first > 0) e = first_float(S.lo, max, [&](float f) { return S.bin(f) < first; });
+            else e = (float)FKeys::value(FKeys::of(__float_as_uint(max)) + 1);       // (the next float: above it all is listed)
         }
         if ((tid & 63) == 0) L.edge[wave] = e;
     }
