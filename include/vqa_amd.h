@@ -500,7 +500,7 @@ int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlo
  *   Kept: the first top_k tokens; of these those with w >= min_p ((x - max) / temperature >= log min_p); of these the tokens whose exclusive cumulative weight is
  *   below top_p times their total.  Drawn: the first kept token whose inclusive cumulative weight exceeds u times the kept
  *   weight.  logp: log of its weight over the kept weight.
- * Weights are exp in 64 bits rounded to a multiple of 2^-s, s = min(51, 62 - ceil(log2 V)), their sums exact: the same
+ * Weights are exp in 64 bits, their sums exact or in a fixed order and within 2^-42 of the weights they stand for: the same
  * answer on every run.  -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw
  * gets token -1 and logp -inf.  temperature <= 0 or NaN: the first token of the order, logp 0.  top_k <= 0, top_p >= 1, min_p <= 0
  * (or NaN): off; top_p <= 0 or NaN, min_p >= 1: the first token, and with min_p its equals.  u below 0 or NaN counts as 0,

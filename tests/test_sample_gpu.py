@@ -263,7 +263,7 @@ def test_lists_of_every_length(dtype, V):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [16384, 20011])
+@pytest.mark.parametrize('V', [8192, 20011])
 def test_rows_whose_parts_differ(dtype, V):
     """Long rows are laid out by what a sixteenth of them shows: rows that rise or fall, whose front is masked, constant or
     narrow, with a few or many tokens above and below everything in front of them."""

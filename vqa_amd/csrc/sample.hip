@@ -5,15 +5,22 @@
 // whose exclusive cumulative weight is below top_p times the weight of what the other two keep), so all together do.  The
 // answer is the first token whose inclusive cumulative weight exceeds u times the kept weight.
 //
-// Nothing is sorted.  A weight is an integer, w rounded to a multiple of 2^-s with V 2^s < 2^63, and a function of the logit
-// alone: sums are exact and the same in any order, atomics included.  Each of the three questions - the k-th token, the last
-// token of the nucleus, the drawn one - asks which token of the order holds place t, counted in tokens or in weight; a
-// radix search over order-preserving integer keys answers it: a histogram of the keys' leading bits (tokens and weight per
-// bin, in LDS), the bin that holds t, a histogram of the next bits of that bin's keys, and so on to a single key; equal keys
-// weigh the same, so the place among them is a division.
-//
 // exp is evaluated in 64 bits: a draw compares sums of up to V weights with u times their sum, and with fp32 exponentials
-// (2^-22) one row in ten of a flat distribution over 10^5 tokens would get a neighbouring token.
+// (2^-22) one row in ten of a flat distribution over 10^5 tokens would get a neighbouring token.  Weights that are summed by
+// atomics are integers, w rounded to a multiple of 2^-s with V 2^s < 2^63: sums are exact, the same in any order.
+//
+// No row is sorted.  Each of the three questions - the k-th token, the last token of the nucleus, the drawn one - asks which
+// token of the order holds a place, counted in tokens or in weight.  Three kernels by the size of the vocabulary:
+//   V <= 64    sample_wave_kernel: a wave a row, a token a lane, every lane looks at all others (1024 x 44: 4.7 us)
+//   V <= 128   sample_list_kernel: a workgroup a row, all tokens in a short sorted list (1024 x 100: 7.5 us)
+//   above      sample_row_kernel: a histogram over steps of the logit finds the bins in which the answers lie, and only their
+//              tokens are listed and sorted.  Bound by the histogram's 64-bit arithmetic, 9 such operations a logit at about 7
+//              cycles a wave: 512 x 131072 take 39 us of it on 256 units, next to 54 us for reading fp32 logits once and 27 for
+//              reading them from the last-level cache to list them (107 us in all, 2.5 TB/s).
+// radix_row takes what those lists cannot hold: rows with thousands of equal logits around an answer.  It goes by the bits of
+// order-preserving integer keys: a histogram of the leading ones (tokens and weight per bin, in LDS), the bin that holds the
+// place, a histogram of the next bits of that bin's keys, and so on to a single key; equal keys weigh the same, so the place
+// among them is a division.
 #include "rows.h"
 #include <float.h>
 
@@ -410,18 +417,18 @@ template <int DT, int BT, int RB> __device__ __attribute__((noinline)) void radi
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
-// 64 < V <= LIST_ALL: every token goes on the list.  Above: three passes over the row -
-//   1. its maximum and minimum;
+// 64 < V <= LIST_ALL: every token goes on the list.  Above:
+//   1. the row's maximum and minimum, or a guess of them;
 //   2. a histogram over BINS equal steps of x below the maximum, down to where weights no longer count (e^-WINDOW).  With
 //      top-k, of tokens: the list is what is not below the k-th token's bin.  Without, of weight: a token of bin b weighs
-//      e^(-b d) e^(-f d) with |f| <= 1/2 and d <= 0.01, the second factor is a short polynomial (off by 2^-45 at most) and
-//      added as an integer; the bin's weight is that sum times e^(-b d), and a scan gives the weight in front of each bin;
+//      e^(-b d) e^(-(f - 1/2) d) with 0 <= f < 1, the second factor is a short polynomial and added as an integer; the bin's
+//      weight is that sum times e^(-b d), and a scan gives the weight in front of each bin;
 //   3. the list: the tokens of the bin that the nucleus ends in and of the bins that the draw can fall into.
 // The list (key and index of each token, LIST at most) is sorted in LDS, its weights are added up in order, and nucleus and
 // draw are looked up in it.  Rows whose list would be too long - many equal logits - go to the radix search.
 #define LIST_ALL 128
 #define WINDOW 40.0
-#define GUESS_FROM 16384
+#define GUESS_FROM 8192
 
 typedef Keys<VQA_F32> FKeys;       // the list's keys: of the logits as fp32, whatever their type
 
@@ -753,7 +760,8 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     // The maximum of a whole row costs a pass over memory in which little is computed, and the histogram is bound by
     // arithmetic.  Without min-p (which needs the true maximum) long rows take both passes as one: the bins lie between the
     // largest and the smallest logit of a sixteenth of the row, and the few tokens outside go on the list at once.  If they
-    // are not few, it starts again with the whole row's.
+    // are not few, it starts again with the whole row's.  (512 x 131072 fp32, top-p: 143 us in two passes, 107 in one;
+    // 1024 x 16000 bf16 50 and 44, 1024 x 4096 22.7 and 22.9.)
     bool guess = PHASE == WHOLE && P.V >= GUESS_FROM && !(r.min_p > 0.0);
     float max, min;
     Weights<VQA_F32> W;
@@ -849,21 +857,25 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
                 }
             };
             if (by_count) {
-                H.template each<2>([&](float f, int i) {
+                H.template each<4>([&](float f, int i) {
                     if ((f >= lo) & (f <= max)) atomicAdd((uint32_t*)&B.mass[S.bin(f)], 1u);
                     else if (PHASE == WHOLE) outside(f, i);
                 });
             } else {
                 // e^(-(f - 1/2) d) for 0 <= f < 1: the series around 1/2, in powers of f (and `magic` on top)
                 const double c1 = -d, c2 = d * d * 0.5, c3 = d * d * d * (-1.0 / 6.0), c4 = d * d * d * d * (1.0 / 24.0);
-                const double a3 = uniform(c3 - 2.0 * c4), a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4);
-                const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4);
-                const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 + W.magic);
+                constexpr bool FIFTH = BINS < 4096;          // (d / 2)^5 / 5! is 2^-45 with 4096 bins, 2^-35 with 1024
+                const double c5 = FIFTH ? d * d * d * d * d * (-1.0 / 120.0) : 0.0;
+                const double a4 = uniform(c4 - 2.5 * c5), a3 = uniform(c3 - 2.0 * c4 + 2.5 * c5);
+                const double a2 = uniform(c2 - 1.5 * c3 + 1.5 * c4 - 1.25 * c5);
+                const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4 + 0.3125 * c5);
+                const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 - 0.03125 * c5 + W.magic);
                 const long long magic = __double_as_longlong(W.magic);
-                H.template each<2>([&](float f, int i) {
+                H.template each<4>([&](float f, int i) {
                     if ((f >= lo) & (f <= max)) {
                         const double a = S.at(f), e = __builtin_amdgcn_fract(a);
-                        const double p = fma(e, fma(e, fma(e, fma(e, c4, a3), a2), a1), a0);
+                        const double q = FIFTH ? fma(e, c5, a4) : a4;
+                        const double p = fma(e, fma(e, fma(e, fma(e, q, a3), a2), a1), a0);
                         atomicAdd(&B.mass[(uint32_t)a], (unsigned long long)(__double_as_longlong(p) - magic));
                     } else if (PHASE == WHOLE) {
                         outside(f, i);

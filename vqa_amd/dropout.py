@@ -34,7 +34,7 @@ class _Dropout(torch.autograd.Function):
         x = x.contiguous()
         y = torch.empty_like(x)
         ops.dropout(x, y, thr, seed, offset, state)
-        ctx.args = thr, seed, offset
+        ctx.args = thr, seed & 2 ** 64 - 1, offset & 2 ** 64 - 1
         ctx.save_for_backward(state)          # (changed before backward, it would give another mask: autograd refuses that)
         return y
 
@@ -48,7 +48,7 @@ def _dropout_grad(ctx, dy):
     (state,) = ctx.saved_tensors
     dy = dy.contiguous()
     dx = torch.empty_like(dy)
-    ops.dropout(dy, dx, *ctx.args, state)
+    ops.dropout_backward(dy, dx, *ctx.args, state)
     return dx, None, None, None, None
 
 

@@ -418,8 +418,14 @@ def dropout(x, y, threshold, seed, offset, state=None):
     _same_device(x, y, state)
     assert x.dtype == y.dtype and x.is_contiguous() and y.is_contiguous() and y.numel() >= x.numel()
     assert state is None or (state.dtype == torch.int64 and state.is_contiguous() and state.numel() == 2)
-    _call_on(x, _lib.load().vqa_dropout, x.data_ptr(), y.data_ptr(), x.numel(), ROW_DTYPES[x.dtype], threshold, seed & 2 ** 64 - 1,
-             offset & 2 ** 64 - 1, _addr(state))
+    dropout_backward(x, y, threshold, seed & 2 ** 64 - 1, offset & 2 ** 64 - 1, state)
+
+
+def dropout_backward(dy, dx, threshold, seed, offset, state):
+    """The same on the gradient (seed and offset in [0, 2^64)).  Shapes and types are the caller's care here: this runs in
+    autograd's thread, where the checks above take 8 us."""
+    _call_on(dy, _lib.load().vqa_dropout, dy.data_ptr(), dx.data_ptr(), dy.numel(), ROW_DTYPES[dy.dtype], threshold, seed, offset,
+             _addr(state))
 
 
 def slot_sum_mask(arena, blob, off_offsets, off_src, off_dst, off_mask, n_dst, slot_elems):
