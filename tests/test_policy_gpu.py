@@ -1,5 +1,5 @@
 """The operators of the program policy where the framework uses them: dropout on the executor's hidden layers, and a whole
-round of sampling programs on the device, scoring them, and training the generator and the executor on the outcome."""
+cycle of sampling programs on the device, scoring them, and training the generator and the executor on the outcome."""
 import numpy as np
 import pytest
 import torch

@@ -2,7 +2,6 @@
 import ctypes as C
 import math
 
-import numpy as np
 import pytest
 import torch
 
@@ -11,7 +10,7 @@ from vqa_amd import _lib, dropout, loss, ops, sampling
 
 
 def test_generator_known_answers():
-    """Vectors published with the generator (Random123, kat_vectors: philox4x32 10)."""
+    """Vectors published with the generator."""
     pi = [0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344]
     for ctr, key, want in (([0] * 4, [0] * 2, '6627e8d5 e169c58d bc57ac4c 9b00dbd8'),
                            ([2 ** 32 - 1] * 4, [2 ** 32 - 1] * 2, '408f276d 41c83b0e a20bc7c6 6d5451fd'),
@@ -131,4 +130,20 @@ def test_c_entry_refusals():
 
 def test_struct_matches_the_header():
     assert C.sizeof(_lib.SampleParams) == 9 * 8 + 3 * 8 + 3 * 8 + 4 * 4
-    assert np.dtype('f8').itemsize == 8
+
+
+def test_hidden_dropout_takes_its_counters_and_ranks_differ(vocab, monkeypatch):
+    from vqa_amd.module_net import ModuleNet
+    net = ModuleNet(False, vocab, feature_dim=(128, 14, 14), classifier_proj_dim=128, classifier_fc_layers=(256, 128))
+    assert net._start_dropout(5) is None
+    net.hidden_dropout, net.dropout_seed, net.dropout_offset = 0.25, 7, 10
+    assert net._start_dropout(5) == (16384, 7, [10, 10 + 160])
+    assert net.dropout_offset == 10 + 160 + 80
+    monkeypatch.setattr(torch.distributed, 'is_initialized', lambda: True)
+    monkeypatch.setattr(torch.distributed, 'get_rank', lambda: 3)
+    assert net._start_dropout(5)[1] == 10
+    net.eval()
+    assert net._start_dropout(5) is None
+    net.hidden_dropout = -0.1
+    with pytest.raises(ValueError):
+        net._start_dropout(5)

@@ -73,7 +73,7 @@ def uniform(rows, seed):
     return torch.rand(rows, generator=torch.Generator().manual_seed(seed))
 
 
-SIZES = [(3, 1), (5, 2), (40, 44), (9, 64), (9, 65), (6, 300), (5, 1023), (5, 2049), (4, 8192), (4, 8193), (3, 50001), (2, 131072)]
+SIZES = [(3, 1), (5, 2), (40, 44), (9, 64), (9, 65), (7, 100), (7, 128), (7, 129), (6, 300), (5, 1023), (5, 2049), (4, 8192), (4, 8193), (3, 50001), (2, 131072)]
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
@@ -116,7 +116,7 @@ def test_parameters_outside_their_range_in_a_tensor(V):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('V', [44, 64, 300, 9001, 50009])
+@pytest.mark.parametrize('V', [44, 64, 100, 300, 9001, 50009])
 def test_masks_infinities_and_nan(dtype, V):
     x = logits(12, V, V, dtype)
     x[0, :] = -math.inf
@@ -144,9 +144,14 @@ def test_ties_go_by_index(dtype, V):
     x[1, V // 3:] = 1.0
     x[2, ::2] = 1.0
     x[3, 1::3] = -2.0
+    from vqa_amd.sampling import sample
     for u in (0.0, 0.25, 0.5, 0.999):
         for params in (dict(), dict(top_k=5), dict(top_k=V - 2), dict(top_p=0.5), dict(top_p=0.37, top_k=V // 2)):
             check(x, torch.full((4,), u), **params)
+            # and in a batch of more rows, which other kernels do
+            us = torch.full((300,), u, device=dev())
+            many = sample(x.repeat(75, 1), us, **params)
+            assert torch.equal(many.view(75, 4), sample(x, us[:4], **params).expand(75, 4))
 
 
 def test_frequencies_over_all_numbers():
@@ -188,7 +193,7 @@ def test_more_rows_than_workgroups():
     check(x[:64], u[:64].cpu())
 
 
-@pytest.mark.parametrize('V', [2000, 20000, 100003])
+@pytest.mark.parametrize('V', [2000, 12000, 20000, 100003])
 def test_the_same_row_in_batches_of_every_size(V):
     """How many rows a call has decides how a row is split and by how many threads it is done: the answers agree."""
     from vqa_amd.sampling import sample
