@@ -258,3 +258,24 @@ def test_saved_tensor_hooks_may_move_what_backward_reads():
         del scratch
     for other in got[1:]:
         assert torch.equal(got[0][0], other[0]) and torch.equal(got[0][1], other[1])
+
+
+def test_saved_tensor_hooks_may_lay_logits_out_anew_at_the_same_address():
+    """An offloaded tensor that comes back can get the address it had: its strides are what tells."""
+    from vqa_amd.loss import token_log_probs
+    tk = tokens_for((3, 5), 101, 1).to(dev())
+    leaf = logits((3, 6, 101), 2, torch.bfloat16).requires_grad_(True)
+    (want,) = torch.autograd.grad(token_log_probs((leaf * 2)[:, :-1], tk).sum(), leaf)
+    moved = []
+
+    def unpack(saved):
+        t, dense = saved
+        if t.is_contiguous():
+            return dense
+        back = t.data.as_strided(dense.shape, dense.stride(), t.storage_offset())
+        moved.append(back.copy_(dense).data_ptr() == t.data_ptr() and back.stride() != t.stride())
+        return back
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (t, t.detach().clone(memory_format=torch.contiguous_format)), unpack):
+        lp = token_log_probs((leaf * 2)[:, :-1], tk)
+    (got,) = torch.autograd.grad(lp.sum(), leaf)
+    assert moved == [True] and torch.equal(got, want)

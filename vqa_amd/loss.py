@@ -63,7 +63,7 @@ class _TokenLogProbs(torch.autograd.Function):
             ops.token_logp(x, layout, tk, lp, ent, stats, x.size(-1), temperature, ignore)
         # (the caller's own tensor where it was read in place: autograd then notices a change before backward)
         ctx.save_for_backward(x, tk, stats)
-        ctx.args = x.data_ptr(), layout, logits.shape, temperature, ignore
+        ctx.args = x.stride(), layout, logits.shape, temperature, ignore
         return (lp, ent) if want_entropy else lp
 
     @staticmethod
@@ -76,8 +76,8 @@ def _log_probs_grad(ctx, g, h):
     if g is None and h is None:
         return None, None, None, None, None
     x, tk, stats = ctx.saved_tensors
-    ptr, layout, shape, temperature, ignore = ctx.args
-    if x.data_ptr() != ptr:                   # (a saved-tensor hook has put it elsewhere, with strides of its own)
+    strides, layout, shape, temperature, ignore = ctx.args
+    if x.stride() != strides:                 # (a saved-tensor hook has laid it out anew, be it at the same address)
         x, *layout = ops.row_layout(x)
     dx = torch.empty(shape, dtype=x.dtype, device=x.device)
     if layout[0]:
