@@ -173,3 +173,20 @@ def test_a_round_of_sampling_scoring_and_training(vocab):
     loss.backward()
     assert net.dropout_offset > before and np.isfinite(loss.item())
     assert all(torch.isfinite(p.grad).all() for p in net.parameters() if p.grad is not None)
+
+
+def test_saved_tensors_left_on_the_host_are_refused():
+    """A saved-tensor hook that moves to the host and does not move back."""
+    from vqa_amd.dropout import dropout
+    from vqa_amd.loss import token_log_probs
+    x = torch.randn(4, 44, device='cuda:0', requires_grad=True)
+    tk = torch.zeros(4, dtype=torch.int64, device='cuda:0')
+    state = torch.tensor([1, 2], dtype=torch.int64, device='cuda:0')
+    for left in (lambda t: True, lambda t: t.dtype == torch.int64, lambda t: t.numel() == 16):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu() if left(t) else t, lambda t: t):
+            lp, y = token_log_probs(x, tk), dropout(x, 0.5, state)
+        with pytest.raises(RuntimeError, match='no CPU fallback'):
+            lp.sum().backward()
+        if left(state):
+            with pytest.raises(RuntimeError, match='no CPU fallback'):
+                y.sum().backward()

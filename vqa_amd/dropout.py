@@ -46,6 +46,8 @@ class _Dropout(torch.autograd.Function):
 def _dropout_grad(ctx, dy):
     # (as little as can be: what runs in autograd's thread takes three times as long as in the caller's)
     (state,) = ctx.saved_tensors
+    if state is not None and state.get_device() != dy.get_device():
+        ops._same_device(dy, state)           # (raises: a saved-tensor hook has left it elsewhere)
     dy = dy.contiguous()
     dx = torch.empty_like(dy)
     ops.dropout_backward(dy, dx, *ctx.args, state)

@@ -76,6 +76,8 @@ def _log_probs_grad(ctx, g, h):
     if g is None and h is None:
         return None, None, None, None, None
     x, tk, stats = ctx.saved_tensors
+    if not x.get_device() == tk.get_device() == stats.get_device():
+        ops._same_device(x, tk, stats)        # (raises: a saved-tensor hook has left some elsewhere)
     strides, layout, shape, temperature, ignore = ctx.args
     if x.stride() != strides:                 # (a saved-tensor hook has laid it out anew, be it at the same address)
         x, *layout = ops.row_layout(x)

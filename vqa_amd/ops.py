@@ -333,6 +333,8 @@ def _call_on(t, fn, *args):
     """fn(*args, stream) with t's device as the current one and its current stream.  (Both are asked for directly:
     torch.cuda.current_stream() takes 28 us in autograd's threads.)"""
     i = t.get_device()
+    if i < 0:
+        _need_cuda(t)
     if i == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
