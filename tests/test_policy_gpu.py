@@ -190,3 +190,17 @@ def test_saved_tensors_left_on_the_host_are_refused():
         if left(state):
             with pytest.raises(RuntimeError, match='no CPU fallback'):
                 y.sum().backward()
+
+
+def test_tokens_written_over_before_backward_are_refused():
+    from vqa_amd.loss import token_log_probs
+    from vqa_amd.sampling import sample
+    x = torch.randn(4, 44, device='cuda:0', requires_grad=True)
+    u, tk = torch.rand(4, device='cuda:0'), torch.zeros(4, dtype=torch.int64, device='cuda:0')
+    lp = token_log_probs(x, tk)
+    sample(x, u, out=tk)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        lp.sum().backward()
+    with torch.inference_mode():
+        out = torch.zeros(4, dtype=torch.int64, device='cuda:0')
+        assert torch.equal(sample(x, u, out=out), tk)

@@ -62,4 +62,6 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     logp = torch.empty(rows, dtype=torch.float32, device=dev) if return_log_probs else None
     if rows:
         ops.sample(x, x.stride(0), rows, V, u if u.is_contiguous() else u.contiguous(), token, token.stride(0), logp, *params)
+        if out is not None:                   # as every write in place: tokens that a backward pass still needs are missed then
+            torch.autograd.graph.increment_version(out)
     return (token, logp) if return_log_probs else token
