@@ -294,3 +294,15 @@ def test_rows_whose_parts_differ(dtype, V):
                    dict(temperature=0.05, top_p=0.9), dict(temperature=20.0), dict(min_p=0.01), dict(temperature=0.0)):
         for u in (0.0, 0.3, 0.8, 1 - 2.0 ** -24):
             check(x, torch.full((14,), u), **params)
+
+
+@pytest.mark.parametrize('V', [44, 100, 700, 12000, 70000])
+def test_the_smallest_temperatures(V):
+    """Down to numbers whose reciprocal is infinite: the largest logits share all the weight."""
+    x = logits(6, V, V, torch.float32)
+    x[1, 3:9] = x[1].max()
+    x[2, ::2] = 40.0
+    x[3] = torch.arange(V, device=dev()) * 1e-45
+    for t in (5e-324, 1e-310, 1e-290, 1e-45):
+        for params in (dict(), dict(top_p=0.6), dict(top_k=3), dict(min_p=0.1)):
+            check(x, uniform(6, V), temperature=t, **params)

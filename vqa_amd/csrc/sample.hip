@@ -127,6 +127,7 @@ __device__ __forceinline__ RowParams row_params(const SampleArgs& P, int64_t row
         r.t = 1.0;
         r.k = 1;
     }
+    r.t = r.t > 1e-290 ? r.t : 1e-290;                       // (1 / t is finite; floats that differ are 1e-45 apart or more)
     return r;
 }
 template <int DT> __device__ __forceinline__ Weights<DT> row_weights(const RowParams& r, uint32_t top, int shift) {
