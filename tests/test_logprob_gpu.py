@@ -279,3 +279,11 @@ def test_saved_tensor_hooks_may_lay_logits_out_anew_at_the_same_address():
         lp = token_log_probs((leaf * 2)[:, :-1], tk)
     (got,) = torch.autograd.grad(lp.sum(), leaf)
     assert moved == [True] and torch.equal(got, want)
+
+
+def test_an_ignore_index_outside_the_vocabulary_matches_nothing():
+    from vqa_amd.loss import token_log_probs
+    x, tk = logits((8, 44), 1, torch.float32), torch.arange(8, device=dev())
+    want = token_log_probs(x, tk)
+    for i in (None, -100, 44, 2 ** 32, 2 ** 63, 2 ** 64, 2 ** 64 + 3, -2 ** 64):
+        assert torch.equal(token_log_probs(x, tk, ignore_index=i), want)

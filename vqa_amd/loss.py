@@ -106,5 +106,5 @@ def token_log_probs(logits, tokens, temperature=1.0, ignore_index=None, entropy=
     if not 1e-6 <= temperature <= 1e6:
         raise ValueError('temperature must be in [1e-6, 1e6]')
     ops._same_device(logits, tokens)
-    ignore = -1 if ignore_index is None else int(ignore_index)
+    ignore = -1 if ignore_index is None or not 0 <= ignore_index < logits.size(-1) else int(ignore_index)
     return _TokenLogProbs.apply(logits, tokens, temperature, ignore, bool(entropy))
