@@ -147,3 +147,16 @@ def test_hidden_dropout_takes_its_counters_and_ranks_differ(vocab, monkeypatch):
     net.hidden_dropout = -0.1
     with pytest.raises(ValueError):
         net._start_dropout(5)
+
+
+def test_hidden_dropout_is_refused_in_a_captured_graph(vocab, monkeypatch):
+    from vqa_amd.module_net import ModuleNet
+    net = ModuleNet(False, vocab, feature_dim=(128, 14, 14), classifier_proj_dim=128, classifier_fc_layers=(256, 128))
+    monkeypatch.setattr(torch.cuda, 'is_available', lambda: True)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    assert net._start_dropout(5) is None
+    net.hidden_dropout = 0.25
+    with pytest.raises(RuntimeError, match='counts on the host'):
+        net._start_dropout(5)
+    assert net.dropout_offset == 0
+    assert net.eval()._start_dropout(5) is None
