@@ -160,3 +160,16 @@ def test_hidden_dropout_is_refused_in_a_captured_graph(vocab, monkeypatch):
         net._start_dropout(5)
     assert net.dropout_offset == 0
     assert net.eval()._start_dropout(5) is None
+
+
+def test_a_module_pickled_without_hidden_dropout_still_runs(vocab):
+    import pickle
+
+    from vqa_amd.module_net import ModuleNet
+    net = ModuleNet(False, vocab, feature_dim=(128, 14, 14), classifier_proj_dim=128, classifier_fc_layers=(256, 128))
+    for name in ('hidden_dropout', 'dropout_seed', 'dropout_offset'):
+        net.__dict__.pop(name, None)
+    net = pickle.loads(pickle.dumps(net))
+    assert net._start_dropout(5) is None and net.dropout_offset == 0
+    net.hidden_dropout = 0.5
+    assert net._start_dropout(5) == (32768, 0, [0, 160])

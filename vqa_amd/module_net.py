@@ -76,6 +76,15 @@ class _ExecFn(torch.autograd.Function):
 
 
 class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
+    # dropout on every hidden layer of the classifier (behind its ReLU) while the module is in training mode: the
+    # opt-in for the reference's classifier_dropout, under the default network's state-dict keys.  Masks come from
+    # vqa_amd.dropout: a function of dropout_seed (plus the data-parallel rank) and dropout_offset, which every
+    # such call advances; nothing is stored for backward.  (Of the class:
+    # a module pickled before they were there has none)
+    hidden_dropout = 0.0
+    dropout_seed = 0
+    dropout_offset = 0
+
     def __init__(self, info, vocab,
                  feature_dim=(1024, 14, 14),
                  stem_num_layers=2,
@@ -215,13 +224,6 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
         self.backward_order = os.environ.get('VQA_BWD_ORDER', 'A')
         self.schedule_error = None
         self._arity_dev = None
-        # dropout on every hidden layer of the classifier (behind its ReLU) while the module is in training mode: the
-        # opt-in for the reference's classifier_dropout, under the default network's state-dict keys.  Masks come from
-        # vqa_amd.dropout: a function of dropout_seed (plus the data-parallel rank) and dropout_offset, which every
-        # such call advances; nothing is stored for backward
-        self.hidden_dropout = 0.0
-        self.dropout_seed = 0
-        self.dropout_offset = 0
         self.keep_state = False       # tests: keep the last call's buffers in self.last_state
         # list-of-dicts programs: False = the reference's behaviour (AttributeError); True = run them
         self.accept_program_lists = False
