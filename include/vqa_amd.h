@@ -497,11 +497,11 @@ int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlo
  * (Seq2Seq.reinforce_sample, LSTM_Model.py:205-235, which copies every step's tokens to the host), its tokens written
  * straight into a column of the [N][T] int64 program array that vqa_devsched_build reads.
  *   Order: descending logit, equal logits by index.  Weights: w = exp((x - max) / temperature).
- *   Kept: the first top_k tokens; of these those with w >= min_p ((x - max) / temperature >= log min_p); of these the tokens whose exclusive cumulative weight is
- *   below top_p times their total.  Drawn: the first kept token whose inclusive cumulative weight exceeds u times the kept
- *   weight.  logp: log of its weight over the kept weight.
- * Weights are exp in 64 bits, their sums exact or in a fixed order and within 2^-42 of the weights they stand for: the same
- * answer on every run.  -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw
+ *   Kept: the first top_k tokens; of these those with w >= min_p ((x - max) / temperature >= log min_p); of these the tokens
+ *   whose exclusive cumulative weight is below top_p times their total.  Drawn: the first kept token whose inclusive
+ *   cumulative weight exceeds u times the kept weight.  logp: log of its weight over the kept weight.
+ * Weights are exp in 64 bits, those below e^-40 may count as 0; sums are exact or in a fixed order and within 2^-42 of the
+ * weights they stand for: the same answer on every run.  -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw
  * gets token -1 and logp -inf.  temperature <= 0 or NaN: the first token of the order, logp 0.  top_k <= 0, top_p >= 1, min_p <= 0
  * (or NaN): off; top_p <= 0 or NaN, min_p >= 1: the first token, and with min_p its equals.  u below 0 or NaN counts as 0,
  * u >= 1 draws the last kept token.
