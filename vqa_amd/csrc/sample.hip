@@ -510,45 +510,69 @@ __device__ __forceinline__ void raise(uint32_t* out, int v) {
     if (m && (threadIdx.x & 63) == 63 - __clzll((unsigned long long)m)) atomicMax(out, (uint32_t)v);
 }
 
-// Sorts list[0, n), descending; the answer is in `list` or, true, in `other`; both have room for the next power of two.
-// Short lists by counting what is larger than each entry, n * n / BT comparisons a thread without a barrier (n = 256, 1024
-// threads: 1 us); longer ones by a bitonic network, whose barriers cost 0.15 us each (n = 256: 36 of them).
+// Sorts list[0, n), descending; the answer is in `list` or, true, in `other`; both have room for the next multiple of 64.
+// Every wave sorts stretches of 64 in registers, then four sorted runs at a time become one: an entry's place among them is the
+// sum of its places in each, found by three searches that run side by side.  (Not inlined: the kernels keep their registers.)
+template <int BT>
+__device__ __attribute__((noinline)) bool sort_runs(LDS_AS unsigned long long* list, LDS_AS unsigned long long* other, int n) {
+    const int tid = threadIdx.x, lane = tid & 63, m = (n + 63) & ~63;
+    for (int i = tid; i < m; i += BT) {                      // (whole waves: m and i - lane are multiples of 64)
+        unsigned long long e = i < n ? list[i] : 0;
+#pragma unroll
+        for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+            for (int j = k >> 1; j > 0; j >>= 1) {
+                const unsigned long long o = __shfl_xor(e, j);
+                e = ((lane & j) == 0) == ((lane & k) == 0) ? (o > e ? o : e) : (o < e ? o : e);
+            }
+        list[i] = e;
+    }
+    __syncthreads();
+    bool swapped = false;
+    for (int run = 64; run < n; run *= 4) {
+        const LDS_AS unsigned long long* src = swapped ? other : list;
+        LDS_AS unsigned long long* dst = swapped ? list : other;
+        for (int i = tid; i < m; i += BT) {
+            const unsigned long long e = src[i];
+            const int base = i & ~(4 * run - 1), mine = (i - base) / run;
+            int o[3], len[3], at[3] = {0, 0, 0};
+            unsigned long long least[3];                     // equal ones (the padding) keep their order
+#pragma unroll
+            for (int q = 0; q < 3; q++) {
+                const int r = q + (q >= mine);
+                o[q] = base + r * run;
+                len[q] = min(max(m - o[q], 0), run);
+                least[q] = r < mine ? e : e + 1;             // (no key is all ones)
+            }
+            for (int step = run; step > 0; step >>= 1)
+#pragma unroll
+                for (int q = 0; q < 3; q++)
+                    if (at[q] + step <= len[q] && src[o[q] + at[q] + step - 1] >= least[q]) at[q] += step;
+            dst[base + (i - base - mine * run) + at[0] + at[1] + at[2]] = e;
+        }
+        __syncthreads();
+        swapped = !swapped;
+    }
+    return swapped;
+}
+
+// The same; short lists by counting what is larger than each entry, n * n / BT comparisons a thread without a barrier.  (100 x 20000
+// fp32 with 1024 threads, counted against merged: top-k 200 20.7 / 22 us, 300 26 / 23, 500 32 / 25.  A bitonic network in LDS, a
+// barrier at every longer distance, took 31 us where merging takes 25, top-k 700, and as long for the longest lists, 2000.)
 template <int BT> __device__ __forceinline__ bool sort_list(unsigned long long* list, unsigned long long* other, int n) {
     const int tid = threadIdx.x;
-    if (n <= BT / 2) {
-        int parts = 2;                                       // threads an entry
-        while (parts < 64 && parts * 2 * n <= BT) parts *= 2;
-        const int i = tid / parts;
-        const unsigned long long mine = i < n ? list[i] : 0;
-        int rank = 0;
-        if (i < n)
-            for (int j = tid % parts; j < n; j += parts) rank += list[j] > mine;
-        for (int d = 1; d < parts; d <<= 1) rank += __shfl_xor(rank, d);
-        if (i < n && tid % parts == 0) other[rank] = mine;   // (entries differ: so do ranks)
-        __syncthreads();
-        return true;
-    }
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += BT) list[i] = 0;
+    if (n > (BT < 512 ? BT / 2 : 256)) return sort_runs<BT>((LDS_AS unsigned long long*)list, (LDS_AS unsigned long long*)other, n);
+    int parts = 2;                                           // threads an entry
+    while (parts < 64 && parts * 2 * n <= BT) parts *= 2;
+    const int i = tid / parts;
+    const unsigned long long mine = i < n ? list[i] : 0;
+    int rank = 0;
+    if (i < n)
+        for (int j = tid % parts; j < n; j += parts) rank += list[j] > mine;
+    for (int d = 1; d < parts; d <<= 1) rank += __shfl_xor(rank, d);
+    if (i < n && tid % parts == 0) other[rank] = mine;       // (entries differ: so do ranks)
     __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int p = tid; p < size / 2; p += BT) {
-                const int a = 2 * p - (p & (j - 1)), b = a + j;
-                const unsigned long long va = list[a], vb = list[b];
-                if ((va < vb) == ((a & k) == 0)) {
-                    list[a] = vb;
-                    list[b] = va;
-                }
-            }
-            // the pairs of a wave's 64 neighbouring p are its own 128 entries while j <= 64: no other wave touches them
-            // before a step with a larger j (the next one is the next k's first)
-            if (j > 64 || (j == 1 && k >= 128)) __syncthreads();
-            else __builtin_amdgcn_wave_barrier(), __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
-    __syncthreads();
-    return false;
+    return true;
 }
 
 // Nucleus and draw in the sorted list of n tokens.  Without `front` the list holds all that is kept but for the nucleus;
