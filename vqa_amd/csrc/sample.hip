@@ -16,7 +16,7 @@
 //   above      sample_row_kernel: a histogram over steps of the logit finds the bins in which the answers lie, and only their
 //              tokens are listed and sorted.  Bound by the histogram's 64-bit arithmetic, 9 such operations a logit at about 7
 //              cycles a wave: 512 x 131072 take 39 us of it on 256 units, next to 54 us for reading fp32 logits once and 27 for
-//              reading them from the last-level cache to list them (107 us in all, 2.5 TB/s).
+//              reading them from the last-level cache to list them (104 us in all, 2.6 TB/s).
 // radix_row takes what those lists cannot hold: rows with thousands of equal logits around an answer.  It goes by the bits of
 // order-preserving integer keys: a histogram of the leading ones (tokens and weight per bin, in LDS), the bin that holds the
 // place, a histogram of the next bits of that bin's keys, and so on to a single key; equal keys weigh the same, so the place
@@ -1024,8 +1024,9 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
 }
 
 // Workgroups of a row.  A split row pays for three launches and for a scan of its bins in each workgroup of the last: worth it
-// from 32768 logits on for a single row, from 98304 for 64 of them (bf16, top-p 0.9, split against whole: 1 x 50001 23 / 27 us,
-// 1 x 131072 26 / 51, 8 x 65536 32 / 36, 64 x 65536 42 / 36, 64 x 131072 52 / 56), not with more rows (128 x 131072 63 / 59).
+// from 32768 logits on for a single row, from 98304 for 64 of them (bf16, top-p 0.9, split against whole in us: 1 x 50001 24 / 28,
+// 1 x 131072 27 / 46, 8 x 65536 29 / 36, 32 x 65536 37 / 36, 64 x 65536 40 / 37, 64 x 131072 45 / 54), not with more rows
+// (128 x 131072 60 / 54).
 static int sample_parts(int64_t rows, int32_t V) {
     if (rows <= 0 || rows > 64 || V < 32768 + 1024 * rows) return 1;
     const int64_t by_rows = 256 / rows, by_size = V / 8192;
