@@ -306,3 +306,24 @@ def test_the_smallest_temperatures(V):
     for t in (5e-324, 1e-310, 1e-290, 1e-45):
         for params in (dict(), dict(top_p=0.6), dict(top_k=3), dict(min_p=0.1)):
             check(x, uniform(6, V), temperature=t, **params)
+
+
+@pytest.mark.parametrize('rows,V', [(300, 3000), (300, 20000), (4, 20000), (4, 70000)])
+def test_lists_around_the_lengths_of_sorted_runs(rows, V):
+    """Top-k lists of one to thirty-two runs of 64 and a few more, in the kernels of 256, 512 and 1024 threads and in split
+    rows; u all over [0, 1), so that every part of the sorted list is looked up."""
+    from vqa_amd.sampling import sample
+    g = torch.Generator().manual_seed(V + rows)
+    x = torch.randn(4, V, generator=g) * 0.7
+    x[1] = torch.randperm(V, generator=g) * 1e-4                       # no ties
+    x[2] = torch.randint(0, 400, (V,), generator=g) * 0.01             # many
+    x = x.to(dev()).repeat(rows // 4, 1)
+    u = torch.tensor([0.0, 0.25, 0.5, 0.999]).repeat(rows // 4)
+    for k in (63, 65, 128, 129, 255, 256, 257, 320, 511, 512, 513, 577, 1023, 1024, 1025, 1100, 1500, 1999):
+        for shift in range(4):
+            at = u.roll(shift)
+            tk, lp = sample(x, at.to(dev()), top_k=k, return_log_probs=True)
+            for r in range(4):
+                want, logp = draw_row(x[r].double().cpu().numpy(), float(at[r]), top_k=k)
+                assert tk[r].item() == want, (k, r, shift)
+                assert abs(lp[r].item() - logp) <= abs(logp) * 2.0 ** -24 + 1e-12
