@@ -76,4 +76,7 @@ template <int DT> __device__ __forceinline__ u32x4 vec_make(const float* f) {
     return v;
 }
 
+// waits until what this wave has stored (and loaded) before has arrived, atomic stores at the scope that they were made for
+__device__ __forceinline__ void wait_for_stores() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 static inline bool rows_dtype_ok(int32_t dt) { return dt == VQA_BF16 || dt == VQA_F16 || dt == VQA_F32; }

@@ -999,11 +999,13 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     if (SPLIT) {                                             // add them to the row's list; the last workgroup takes it
         if (tid == 0) L.last = atomicAdd(&Q->n, (uint32_t)n);
         __syncthreads();
-        // (entries as atomic stores, and one release a workgroup: a fence by every wave writes the L2 cache back each time,
-        // 43 us for 256 workgroups)
+        // Entries are stored past the L2 cache (atomic, agent scope).  Every wave waits for its own stores before the barrier,
+        // which waits for none, as the release of thread 0 waits for those of its own wave only.  (A fence by every wave would
+        // write the L2 cache back each time, 43 us for 256 workgroups.)
         for (int i = tid; i < n; i += BT)
             if (i < LIST && L.last + i < LIST)
                 __hip_atomic_store(&Q->list[L.last + i], L.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        wait_for_stores();
         __syncthreads();
         if (tid == 0) L.pick = __hip_atomic_fetch_add(&Q->done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
