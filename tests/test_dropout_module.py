@@ -1,0 +1,58 @@
+"""The Dropout module's random numbers: which seed and counters each call takes.  The kernels' place is taken by the generator's
+definition on the CPU, so none of it needs a GPU."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from philox_oracle import bits16
+from vqa_amd import dropout, ops
+
+
+@pytest.fixture(autouse=True)
+def on_the_cpu(monkeypatch):
+    def apply(x, y, threshold, seed, offset, state=None):
+        if state is not None:
+            seed, offset = state.tolist()
+        keep = torch.from_numpy(bits16(x.numel(), seed, offset) >= threshold).view(x.shape)
+        y.copy_(torch.where(keep, x * (65536.0 / (65536 - threshold)), 0.0))
+    monkeypatch.setattr(ops, '_need_cuda', lambda *t: None)
+    monkeypatch.setattr(ops, 'dropout', apply)
+    monkeypatch.setattr(ops, 'dropout_backward', apply)
+
+
+def test_modules_without_a_seed_draw_masks_of_their_own():
+    x = torch.ones(512)
+    a, b = dropout.Dropout(0.5), dropout.Dropout(0.5)
+    torch.manual_seed(3)
+    ya, yb, yc = a(x), b(x), a(x)
+    # two independent masks agree in 256 of 512 elements, give or take 11.3: 8 deviations
+    for u, v in ((ya, yb), (ya, yc), (yb, yc)):
+        assert 166 <= (u == v).sum() <= 346
+    torch.manual_seed(3)                                       # torch's generator decides them
+    assert torch.equal(a(x), ya) and torch.equal(b(x), yb)
+    assert 'seed' not in repr(a) and 'seed=4' in repr(dropout.Dropout(0.5, 4))
+
+
+def test_ranks_draw_masks_of_their_own(monkeypatch):
+    x, drop = torch.ones(512), dropout.Dropout(0.5)
+    got = []
+    monkeypatch.setattr(torch.distributed, 'is_initialized', lambda: True)
+    for rank in range(2):
+        monkeypatch.setattr(torch.distributed, 'get_rank', lambda: rank)
+        torch.manual_seed(3)
+        got.append(drop(x))
+    assert 166 <= (got[0] == got[1]).sum() <= 346
+
+
+@pytest.mark.parametrize('reentrant', [True, False])
+def test_a_recomputed_module_takes_the_same_mask(reentrant):
+    """Activation recomputation runs the forward pass again inside the backward one, with the generator's old state."""
+    torch.manual_seed(5)
+    drop = dropout.Dropout(0.5)
+    w = torch.rand(64, requires_grad=True)
+    x = (torch.rand(64) + 1).requires_grad_(True)
+    out = checkpoint(lambda t: drop(t) * w, x, use_reentrant=reentrant)
+    drop(x.detach())                                           # (another call in between)
+    out.sum().backward()
+    dropped = out.detach() / (x * w).detach()                  # 0 or 2
+    assert torch.allclose(x.grad, dropped * w.detach(), rtol=1e-6) and torch.allclose(w.grad, dropped * x.detach(), rtol=1e-6)

@@ -2,7 +2,7 @@
 and again in the backward pass, and never stored.
 
     y = vqa_amd.dropout.dropout(x, 0.1, seed, offset)          # the caller's own counter
-    drop = vqa_amd.dropout.Dropout(0.1, seed=7)                # or a module that counts; y = drop(x)
+    drop = vqa_amd.dropout.Dropout(0.1)                        # or a module; y = drop(x)
 
 Element i (row-major) is dropped with probability p, rounded to a multiple of 2^-16; the others are multiplied by
 1 / (1 - p) for that rounded p.  Dropped elements become 0 whatever they were.  A call uses the counters offset to
@@ -73,24 +73,39 @@ def dropout(x, p, seed, offset=0):
     return _Dropout.apply(x, thr, int(seed), int(offset), state)
 
 
-class Dropout(torch.nn.Module):
-    """Dropout with a counter of its own: every training call takes the next range of counters of `seed`."""
+def data_rank():
+    """This process's number among the data-parallel ranks, 0 outside of a process group."""
+    on = torch.distributed.is_available() and torch.distributed.is_initialized()
+    return torch.distributed.get_rank() if on else 0
 
-    def __init__(self, p=0.5, seed=0):
+
+class Dropout(torch.nn.Module):
+    """Dropout as a module.  Without a seed every training call draws its own from torch's generator on the host (and adds the
+    data-parallel rank): modules, calls and ranks have independent masks, torch.manual_seed decides them, a run that restores
+    torch.get_rng_state() repeats none, and activation recomputation, which restores that state as well, gets the mask of the
+    first pass.
+
+    With a seed the module counts: every training call takes the next range of counters of that seed, from `offset` on.  Modules
+    or ranks of the same seed and offset have the same masks, and `offset` is not in the state dict: whoever resumes such a run
+    saves it and sets it again."""
+
+    def __init__(self, p=0.5, seed=None):
         super().__init__()
         threshold(p)
-        self.p, self.seed, self.offset = float(p), int(seed), 0
+        self.p, self.seed, self.offset = float(p), None if seed is None else int(seed), 0
 
     def forward(self, x):
         if not self.training or self.p == 0:
             return x
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
-            # the counter would be a constant of the graph: the same mask on every replay
-            raise RuntimeError('vqa_amd.dropout.Dropout counts on the host: in a captured graph call '
+            # the random numbers would be constants of the graph: the same mask on every replay
+            raise RuntimeError('vqa_amd.dropout.Dropout draws or counts on the host: in a captured graph call '
                                'vqa_amd.dropout.dropout with a {seed, offset} tensor')
+        if self.seed is None:
+            return dropout(x, self.p, torch.empty((), dtype=torch.int64, device='cpu').random_().item() + data_rank())
         y = dropout(x, self.p, self.seed, self.offset)
         self.offset += blocks(x.numel())
         return y
 
     def extra_repr(self):
-        return 'p=%g, seed=%d' % (self.p, self.seed)
+        return 'p=%g' % self.p if self.seed is None else 'p=%g, seed=%d' % (self.p, self.seed)

@@ -690,9 +690,7 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             # the counters would be constants of the graph: the same masks on every replay
             raise RuntimeError('hidden_dropout counts on the host: a captured graph takes the module in eval mode')
-        seed = int(self.dropout_seed)
-        if torch.distributed.is_available() and torch.distributed.is_initialized():
-            seed += torch.distributed.get_rank()
+        seed = int(self.dropout_seed) + dropout.data_rank()
         at = []
         for fo in self._dims['fcs']:
             at.append(self.dropout_offset)
