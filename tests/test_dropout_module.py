@@ -56,3 +56,18 @@ def test_a_recomputed_module_takes_the_same_mask(reentrant):
     out.sum().backward()
     dropped = out.detach() / (x * w).detach()                  # 0 or 2
     assert torch.allclose(x.grad, dropped * w.detach(), rtol=1e-6) and torch.allclose(w.grad, dropped * x.detach(), rtol=1e-6)
+
+
+@pytest.mark.parametrize('reentrant', [True, False])
+def test_a_counting_module_refuses_to_be_recomputed(reentrant):
+    """Its second pass would take the next counters, another mask: wrong gradients."""
+    drop = dropout.Dropout(0.5, seed=7)
+    w = torch.rand(64, requires_grad=True)
+    x = torch.rand(64).requires_grad_(True)
+    out = checkpoint(lambda t: drop(t) * w, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match='recomputed'):
+        out.sum().backward()
+    assert drop.offset == 8
+    drop.eval()
+    checkpoint(lambda t: drop(t) * w, x, use_reentrant=reentrant).sum().backward()
+    assert torch.equal(w.grad, x.detach()) and torch.equal(x.grad, w.detach())

@@ -79,6 +79,11 @@ def data_rank():
     return torch.distributed.get_rank() if on else 0
 
 
+def in_backward():
+    """Whether this thread is inside a backward pass: a forward pass there is an earlier one that is recomputed."""
+    return torch._C._current_graph_task_id() >= 0
+
+
 class Dropout(torch.nn.Module):
     """Dropout as a module.  Without a seed every training call draws its own from torch's generator on the host (and adds the
     data-parallel rank): modules, calls and ranks have independent masks, torch.manual_seed decides them, a run that restores
@@ -87,7 +92,7 @@ class Dropout(torch.nn.Module):
 
     With a seed the module counts: every training call takes the next range of counters of that seed, from `offset` on.  Modules
     or ranks of the same seed and offset have the same masks, and `offset` is not in the state dict: whoever resumes such a run
-    saves it and sets it again."""
+    saves it and sets it again.  A counting module cannot be recomputed (the second pass would count on) and raises."""
 
     def __init__(self, p=0.5, seed=None):
         super().__init__()
@@ -103,6 +108,9 @@ class Dropout(torch.nn.Module):
                                'vqa_amd.dropout.dropout with a {seed, offset} tensor')
         if self.seed is None:
             return dropout(x, self.p, torch.empty((), dtype=torch.int64, device='cpu').random_().item() + data_rank())
+        if in_backward():
+            raise RuntimeError('vqa_amd.dropout.Dropout with a seed counts its calls: recomputed in the backward pass it would '
+                               'have another mask; leave the seed out, or call vqa_amd.dropout.dropout with an offset')
         y = dropout(x, self.p, self.seed, self.offset)
         self.offset += blocks(x.numel())
         return y
