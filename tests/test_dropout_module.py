@@ -71,3 +71,23 @@ def test_a_counting_module_refuses_to_be_recomputed(reentrant):
     drop.eval()
     checkpoint(lambda t: drop(t) * w, x, use_reentrant=reentrant).sum().backward()
     assert torch.equal(w.grad, x.detach()) and torch.equal(x.grad, w.detach())
+
+
+@pytest.mark.parametrize('reentrant', [True, False])
+def test_hidden_dropout_refuses_to_be_recomputed(vocab, reentrant):
+    from vqa_amd.module_net import ModuleNet
+    net = ModuleNet(False, vocab, feature_dim=(128, 14, 14), classifier_proj_dim=128, classifier_fc_layers=(256, 128))
+    net.hidden_dropout = 0.25
+    got = []
+
+    def stand_in(x):
+        got.append(net._start_dropout(5))
+        return x * x
+    x = torch.rand(8).requires_grad_(True)
+    out = checkpoint(stand_in, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match='recomputed'):
+        out.sum().backward()
+    assert len(got) == 1 and net.dropout_offset == 160 + 80
+    net.eval()                                                 # without dropout nothing is refused
+    checkpoint(stand_in, x, use_reentrant=reentrant).sum().backward()
+    assert got[1:] == [None, None] and torch.equal(x.grad, 2 * x.detach())

@@ -21,3 +21,19 @@ def test_a_recomputed_module_takes_the_same_mask(dtype, reentrant):
     assert not torch.equal(mask, (other != 0).to(dtype) * 2)
     assert torch.equal(out, x * w * mask)
     assert torch.equal(x.grad, w * mask) and torch.equal(w.grad, x * mask)
+
+
+def test_an_executor_with_hidden_dropout_refuses_to_be_recomputed(vocab):
+    from test_policy_gpu import batch, executor
+    net = executor(vocab)
+    x, prog, _ = batch(vocab, 5)
+    x.requires_grad_(True)
+    net.hidden_dropout = 0.5
+    out = checkpoint(net, x, prog, use_reentrant=True)
+    with pytest.raises(RuntimeError, match='recomputed'):
+        out.sum().backward()
+    assert net.dropout_offset == 5 * 256 // 8
+    net.hidden_dropout = 0.0
+    (want,) = torch.autograd.grad(net(x, prog).sum(), x)
+    checkpoint(net, x, prog, use_reentrant=True).sum().backward()
+    assert torch.equal(x.grad, want)

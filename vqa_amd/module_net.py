@@ -690,6 +690,8 @@ class ModuleNet(_WeightPacking, _Fp32Path, nn.Module):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             # the counters would be constants of the graph: the same masks on every replay
             raise RuntimeError('hidden_dropout counts on the host: a captured graph takes the module in eval mode')
+        if dropout.in_backward():
+            raise RuntimeError('hidden_dropout counts its calls: recomputed in the backward pass it would have other masks')
         seed = int(self.dropout_seed) + dropout.data_rank()
         at = []
         for fo in self._dims['fcs']:
