@@ -1,5 +1,7 @@
 """The Dropout module's random numbers: which seed and counters each call takes.  The kernels' place is taken by the generator's
 definition on the CPU, so none of it needs a GPU."""
+import threading
+
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
@@ -91,3 +93,19 @@ def test_hidden_dropout_refuses_to_be_recomputed(vocab, reentrant):
     net.eval()                                                 # without dropout nothing is refused
     checkpoint(stand_in, x, use_reentrant=reentrant).sum().backward()
     assert got[1:] == [None, None] and torch.equal(x.grad, 2 * x.detach())
+
+
+def test_two_threads_that_call_one_module_take_different_counters(monkeypatch):
+    drop, took, both = dropout.Dropout(0.5, seed=7), [], threading.Barrier(2, timeout=20)
+
+    def apply(x, y, threshold, seed, offset, state=None):
+        both.wait()                                            # both calls are on their way
+        took.append(offset)
+        y.zero_()
+    monkeypatch.setattr(ops, 'dropout', apply)
+    threads = [threading.Thread(target=drop, args=(torch.ones(64),)) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(took) == [0, 8] and drop.offset == 16

@@ -9,6 +9,8 @@ Element i (row-major) is dropped with probability p, rounded to a multiple of 2^
 offset + ceil(numel / 8) - 1: calls whose ranges do not meet have independent masks, the same range gives the same mask.
 bf16, fp16 or fp32 on the GPU; there is no CPU path.
 """
+import threading
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -84,6 +86,9 @@ def in_backward():
     return torch._C._current_graph_task_id() >= 0
 
 
+_counting = threading.Lock()              # (of the module's, not of an instance: instances are copied and pickled)
+
+
 class Dropout(torch.nn.Module):
     """Dropout as a module.  Without a seed every training call draws its own from torch's generator on the host (and adds the
     data-parallel rank): modules, calls and ranks have independent masks, torch.manual_seed decides them, a run that restores
@@ -111,9 +116,10 @@ class Dropout(torch.nn.Module):
         if in_backward():
             raise RuntimeError('vqa_amd.dropout.Dropout with a seed counts its calls: recomputed in the backward pass it would '
                                'have another mask; leave the seed out, or call vqa_amd.dropout.dropout with an offset')
-        y = dropout(x, self.p, self.seed, self.offset)
-        self.offset += blocks(x.numel())
-        return y
+        with _counting:
+            at = self.offset
+            self.offset = at + blocks(x.numel())
+        return dropout(x, self.p, self.seed, at)
 
     def extra_repr(self):
         return 'p=%g' % self.p if self.seed is None else 'p=%g, seed=%d' % (self.p, self.seed)
