@@ -504,7 +504,7 @@ int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlo
  * weights they stand for: the same answer on every run.  -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw
  * gets token -1 and logp -inf.  temperature <= 0 or NaN: the first token of the order, logp 0.  top_k <= 0, top_p >= 1, min_p <= 0
  * (or NaN): off; top_p <= 0 or NaN, min_p >= 1: the first token, and with min_p its equals.  u below 0 or NaN counts as 0,
- * u >= 1 draws the last kept token.
+ * u >= 1 draws the last kept token that weighs anything.
  * ------------------------------------------------------------------------------------------ */
 typedef struct {
     const void* logits;         /* row r at element r * ld; aligned to an element */

@@ -625,12 +625,14 @@ __device__ __forceinline__ void finish_list(ListShared<CAP>& L, bool swapped, co
         __syncthreads();
         total = L.total;
     }
-    const double t = r.u * total;                            // drawn: the last kept token that does not start behind t
+    // drawn: the last kept token that does not start behind t, of those that weigh anything
+    const double t = r.u * total;
     double g = before;
     int mine = 0;
     for (int i = i0; i < i1 && i <= (int)last; i++) {
-        if (base(i) + g <= t) mine = i;
-        g += weight[i];
+        const double w = weight[i];
+        if (w > 0.0 && base(i) + g <= t) mine = i;
+        g += w;
     }
     raise(&L.pick, mine);
     __syncthreads();
