@@ -500,10 +500,13 @@ int vqa_xent(const float* logits, const int64_t* target, float* loss, float* dlo
  *   Kept: the first top_k tokens; of these those with w >= min_p ((x - max) / temperature >= log min_p); of these the tokens
  *   whose exclusive cumulative weight is below top_p times their total.  Drawn: the first kept token whose inclusive
  *   cumulative weight exceeds u times the kept weight.  logp: log of its weight over the kept weight.
- * Weights are exp in 64 bits, those below e^-40 may count as 0; sums are exact or in a fixed order and within 2^-42 of the
- * weights they stand for: the same answer on every run.  -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw
- * gets token -1 and logp -inf.  temperature <= 0 or NaN: the first token of the order, logp 0.  top_k <= 0, top_p >= 1, min_p <= 0
- * (or NaN): off; top_p <= 0 or NaN, min_p >= 1: the first token, and with min_p its equals.  u below 0 or NaN counts as 0,
+ * Weights are exp in 64 bits.  Where they are summed as integers each is rounded to a multiple of 2^-s,
+ * s = min(51, 62 - ceil(log2 V)): one below 2^-(s + 1) may count as 0 (e^-36 up to 2048 logits, e^-32 at 131072).  A sum is
+ * within V 2^-(s + 1), and 2^-42 of itself, of the sum of its exponentials: 2^-29 of the largest weight at 131072 logits, 2^-23
+ * at 2^20, 2^-3 at the 2^30 that are accepted.  The same answer on every run.
+ * -inf and NaN are never drawn; +inf takes all the weight (shared by several); a row with nothing to draw gets token -1 and
+ * logp -inf.  temperature <= 0 or NaN: the first token of the order, logp 0.  top_k <= 0, top_p >= 1, min_p <= 0 (or NaN): off;
+ * top_p <= 0 or NaN, min_p >= 1: the first token, and with min_p its equals.  u below 0 or NaN counts as 0,
  * u >= 1 draws the last kept token that weighs anything.
  * ------------------------------------------------------------------------------------------ */
 typedef struct {
