@@ -28,8 +28,8 @@ def _per_row(name, v, rows, device):
         if v.shape != (rows,) or v.device != device or v.is_floating_point() != kind.is_floating_point or v.dtype == torch.bool:
             raise ValueError('%s must be a number or a tensor of %d %s on the device of the logits' %
                              (name, rows, 'integers' if name == 'top_k' else 'floating numbers'))
-        if v.dtype == torch.int64:
-            v = v.clamp(0, _RANGES[name][1])
+        if v.dtype in (torch.int64, torch.uint64, torch.uint32):
+            v = v.to(torch.int64).clamp(0, _RANGES[name][1])       # (2^63 and more become negative, then 0: off, as it should)
         return v.detach().to(kind).contiguous()
     lo, hi = _RANGES[name]
     v = int(v) if name == 'top_k' else float(v)
