@@ -19,3 +19,9 @@ def test_top_k_of_every_integer_type(dtype):
     assert got[1] == min(most, 2 ** 31 - 1) or (most > 2 ** 31 and got[1] <= 0)
     if most > 2 ** 33:
         assert check('top_k', torch.tensor([2 ** 32 + 3, 2 ** 31], dtype=dtype)).tolist() == [2 ** 31 - 1] * 2
+
+
+def test_complex_numbers_are_refused():
+    for name in ('temperature', 'top_k', 'top_p', 'min_p'):
+        with pytest.raises(ValueError):
+            check(name, torch.ones(2, dtype=torch.complex64))

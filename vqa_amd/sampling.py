@@ -25,7 +25,8 @@ def _per_row(name, v, rows, device):
     at here: that would wait for the device.  The kernel has an answer for each.)"""
     if isinstance(v, torch.Tensor):
         kind = torch.int32 if name == 'top_k' else torch.float32
-        if v.shape != (rows,) or v.device != device or v.is_floating_point() != kind.is_floating_point or v.dtype == torch.bool:
+        if (v.shape != (rows,) or v.device != device or v.is_floating_point() != kind.is_floating_point or v.dtype == torch.bool or
+                v.is_complex()):
             raise ValueError('%s must be a number or a tensor of %d %s on the device of the logits' %
                              (name, rows, 'integers' if name == 'top_k' else 'floating numbers'))
         if v.dtype in (torch.int64, torch.uint64, torch.uint32):
