@@ -84,7 +84,8 @@ __device__ __forceinline__ void logp_finish(const LogpRows& P, int64_t row, int6
     const bool empty = a.s == 0.f;
     const float xt = elem_get<DT>(logp_row<DT>(P, row) + token);
     const float H = empty ? 0.f : logs - P.inv_t * (a.t / a.s);
-    logp[row] = empty ? -INFINITY : (xt - a.m) * P.inv_t - logs;
+    // (in 64 bits: the difference of two floats may be none, and is one again over the temperature)
+    logp[row] = empty ? -INFINITY : (float)(((double)xt - (double)a.m) * (double)P.inv_t - (double)logs);
     if (entropy) entropy[row] = H;
     stats[row] = make_float4(a.m, logs, H, 0.f);
 }
