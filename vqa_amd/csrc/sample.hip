@@ -704,8 +704,9 @@ template <int DT, int BT> struct RowPass {
             for (int q = 0; q < N; q++) f(vec_get<DT>(r, q), 0);
         }
     }
-    // calls f(x, index) with every logit as a float; U pieces of 16 bytes on their way at a time
-    template <int U, typename F> __device__ __forceinline__ void each(F f) const {
+    // calls f(x, index) with every logit as a float; four pieces of 16 bytes on their way at a time
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        constexpr int U = 4;
         int v = threadIdx.x;
 #pragma unroll 1
         for (; v + (U - 1) * BT < nv; v += U * BT) {
@@ -717,13 +718,11 @@ template <int DT, int BT> struct RowPass {
 #pragma unroll
                 for (int q = 0; q < N; q++) f(vec_get<DT>(r[k], q), (v + k * BT) * N + q);
         }
-        if (U > 1) {
 #pragma unroll 1
-            for (; v < nv; v += BT) {
-                const u32x4 r = vec_load<DT>(x + (int64_t)v * N);
+        for (; v < nv; v += BT) {
+            const u32x4 r = vec_load<DT>(x + (int64_t)v * N);
 #pragma unroll
-                for (int q = 0; q < N; q++) f(vec_get<DT>(r, q), v * N + q);
-            }
+            for (int q = 0; q < N; q++) f(vec_get<DT>(r, q), v * N + q);
         }
 #pragma unroll 1
         for (int i = nv * N + threadIdx.x; i < V; i += BT) f(elem_get<DT>(x + i), i);
@@ -808,7 +807,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
                 min = fminf(min, f >= -FLT_MAX ? f : INFINITY);
             };
             if (guess) H.some(widen);
-            else H.template each<4>(widen);
+            else H.each(widen);
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) {
                 max = fmaxf(max, __shfl_xor(max, d));
@@ -884,7 +883,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
                 }
             };
             if (by_count) {
-                H.template each<4>([&](float f, int i) {
+                H.each([&](float f, int i) {
                     if ((f >= lo) & (f <= max)) atomicAdd((uint32_t*)&B.mass[S.bin(f)], 1u);
                     else if (PHASE == WHOLE) outside(f, i);
                 });
@@ -898,7 +897,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
                 const double a1 = uniform(c1 - c2 + 0.75 * c3 - 0.5 * c4 + 0.3125 * c5);
                 const double a0 = uniform(1.0 - 0.5 * c1 + 0.25 * c2 - 0.125 * c3 + 0.0625 * c4 - 0.03125 * c5 + W.magic);
                 const long long magic = __double_as_longlong(W.magic);
-                H.template each<4>([&](float f, int i) {
+                H.each([&](float f, int i) {
                     if ((f >= lo) & (f <= max)) {
                         const double a = S.at(f), e = __builtin_amdgcn_fract(a);
                         const double q = FIFTH ? fma(e, c5, a4) : a4;
@@ -990,7 +989,7 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     }
     __syncthreads();
     const float e0 = uniform(L.edge[0]), e1 = uniform(L.edge[1]), e2 = uniform(L.edge[2]), e3 = uniform(L.edge[3]);
-    H.template each<4>([&](float f, int i) {
+    H.each([&](float f, int i) {
         if (((f >= e0) & (f < e1)) | ((f >= e2) & (f < e3))) {
             const uint32_t at = atomicAdd(&L.n, 1u);
             if (at < LIST) L.list[at] = list_entry(FKeys::of(__float_as_uint(f)), first_index + i);
