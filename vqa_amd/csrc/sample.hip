@@ -1027,11 +1027,18 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
 }
 
 // Workgroups of a row.  A split row pays for three launches and for a scan of its bins in each workgroup of the last: worth it
-// from 32768 logits on for a single row, from 98304 for 64 of them (bf16, top-p 0.9, split against whole in us: 1 x 50001 24 / 28,
-// 1 x 131072 27 / 46, 8 x 65536 29 / 36, 32 x 65536 37 / 36, 64 x 65536 40 / 37, 64 x 131072 45 / 54), not with more rows
-// (128 x 131072 60 / 54).
+// from 34304 logits on for a single row, from 131072 for 64 of them, not with more rows.  In us, split against whole, of calls one
+// after the other, bf16 / fp32:
+//                  top-p 0.9             top-k 50, top-p 0.95
+//   1 x 50000      23 24 against 28 26   19 20 against 22 21
+//   1 x 131072     25 22 against 45 43   20 20 against 34 34
+//   8 x 65536      28 27 against 32 33   21 21 against 24 27
+//   32 x 65536     37 35 against 36 31   28 29 against 24 25   (whole)
+//   32 x 98304     38 39 against 44 41   30 31 against 31 30
+//   64 x 98304     43 43 against 45 40   33 34 against 30 31   (whole)
+//   64 x 131072    45 48 against 52 50   35 37 against 35 35
 static int sample_parts(int64_t rows, int32_t V) {
-    if (rows <= 0 || rows > 64 || V < 32768 + 1024 * rows) return 1;
+    if (rows <= 0 || rows > 64 || V < 32768 + 1536 * rows) return 1;
     const int64_t by_rows = 256 / rows, by_size = V / 8192;
     const int64_t parts = by_rows < by_size ? by_rows : by_size;
     return (int)(parts < SPLIT_PARTS ? parts : SPLIT_PARTS);
