@@ -11,16 +11,19 @@
 //
 // No row is sorted.  Each of the three questions - the k-th token, the last token of the nucleus, the drawn one - asks which
 // token of the order holds a place, counted in tokens or in weight.  Three kernels by the size of the vocabulary:
-//   V <= 64    sample_wave_kernel: a wave a row, a token a lane, every lane looks at all others (1024 x 44: 4.7 us)
-//   V <= 128   sample_list_kernel: a workgroup a row, all tokens in a short sorted list (1024 x 100: 7.5 us)
+//   V <= 64    sample_wave_kernel: a wave a row, a token a lane, every lane looks at all others
+//   V <= 128   sample_list_kernel: a workgroup a row, all tokens in a short sorted list
 //   above      sample_row_kernel: a histogram over steps of the logit finds the bins in which the answers lie, and only their
-//              tokens are listed and sorted.  Bound by the histogram's 64-bit arithmetic, 9 such operations a logit at about 7
-//              cycles a wave: 512 x 131072 take 39 us of it on 256 units, next to 54 us for reading fp32 logits once and 27 for
-//              reading them from the last-level cache to list them (104 us in all, 2.6 TB/s).
+//              tokens are listed and sorted.  No single bound: 512 x 131072 fp32 logits, top-p 0.95, take 101-106 us.  They issue
+//              28 M vector instructions, 27 a logit, most of them the histogram's 64-bit arithmetic: 46 us of the 1024 SIMDs at
+//              4 cycles each.  LDS accesses that meet in a bank cost 46 k cycles a unit, 19 us.  The row is read twice: 268 MB for
+//              the histogram, 43-50 us by themselves, and again for the list, from the last-level cache (553 MB asked for in all).
 // radix_row takes what those lists cannot hold: rows with thousands of equal logits around an answer.  It goes by the bits of
 // order-preserving integer keys: a histogram of the leading ones (tokens and weight per bin, in LDS), the bin that holds the
 // place, a histogram of the next bits of that bin's keys, and so on to a single key; equal keys weigh the same, so the place
-// among them is a division.
+// among them is a division.  Each of its passes adds two numbers to LDS per logit, and equal ones wait for each other: 512 x 131072
+// bf16 / fp32 take 540 / 680 us at top-k 2100 (top-k 900: 85 / 103), 650 / 910 us with 40 different values, 1.5 / 2.5 ms where all
+// logits are equal; 1 x 50001 135 / 156 us at top-k 2100 (top-k 900: 32 / 33).
 #include "rows.h"
 #include <float.h>
 
@@ -787,7 +790,8 @@ template <int DT, int BT, int BINS, int LIST, SamplePhase PHASE> __global__ __la
     // arithmetic.  Without min-p (which needs the true maximum) long rows take both passes as one: the bins lie between the
     // largest and the smallest logit of a sixteenth of the row, and the few tokens outside go on the list at once.  If they
     // are not few, it starts again with the whole row's.  (512 x 131072 fp32, top-p: 143 us in two passes, 107 in one;
-    // 1024 x 16000 bf16 50 and 44, 1024 x 4096 22.7 and 22.9.)
+    // 1024 x 16000 bf16 50 and 44, 1024 x 4096 22.7 and 22.9.  Where it has to start again: 512 x 131072 fp32 152 us instead of 94,
+    // 1024 x 16000 bf16, whose 2500 raised logits are also too many for the list, 105 instead of 42.)
     bool guess = PHASE == WHOLE && P.V >= GUESS_FROM && !(r.min_p > 0.0);
     float max, min;
     Weights<VQA_F32> W;
@@ -1048,6 +1052,14 @@ extern "C" int64_t vqa_sample_workspace(int64_t rows, int32_t V) {
     return sample_parts(rows, V) > 1 ? rows * (int64_t)sizeof(SplitRow) : 0;
 }
 
+// The kernel of a whole row of more than LIST_ALL logits, in us (calls one after the other, bf16, top-p 0.9):
+//                                      1 x 8192  256 x 4096  256 x 32768  1024 x 4096  1024 x 16384  512 x 65536  1024 x 131072
+//   1024 threads, 4096 bins, list 2048  16        17          27           58           74            71           205
+//   512 threads, 4096 bins, list 2048   16        15          31           36           51            58           168
+//   256 threads, 1024 bins, list 1024   14        14          46           19           37            80           791
+// So: 1024 threads for up to 256 rows, one on a unit, above 4096 logits; 256 threads, whose few bins cost little to scan and of
+// which eight share a unit, up to 16384 logits, above which the tokens of a bin become too many for its list; else 512.
+// The borders are not exact: 257 x 16384 takes 28 us where 512 threads take 25, 4096 x 32768 249 where 256 threads take 196.
 extern "C" int vqa_sample(const vqa_sample_params* p, void* stream) {
     const int size = p && p->dtype == VQA_F32 ? 4 : 2;
     const int parts = p ? sample_parts(p->rows, p->V) : 1;
