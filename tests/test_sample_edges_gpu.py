@@ -43,3 +43,15 @@ def test_weights_of_zero_are_never_drawn(rows, V):
             tk, lp = sample(x, torch.full((rows,), u, device=dev()), return_log_probs=True, **params)
             assert (tk == want).all(), (u, params, tk[:4])
             assert torch.isfinite(lp).all() and (lp > -1.0).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.int8, torch.uint8, torch.int16, torch.uint16, torch.uint32, torch.int64, torch.uint64])
+def test_top_k_in_every_integer_type(dtype):
+    from vqa_amd.sampling import sample
+    x = torch.randn(40, 300, generator=torch.Generator().manual_seed(1)).to(dev())
+    u = torch.rand(40, generator=torch.Generator().manual_seed(2)).to(dev())
+    k = torch.arange(40)
+    assert torch.equal(sample(x, u, top_k=k.to(dtype).to(dev())), sample(x, u, top_k=k.to(torch.int32).to(dev())))
+    if dtype in (torch.int64, torch.uint64):
+        k = torch.full((40,), 2 ** 32 + 3).to(dtype).to(dev())
+        assert torch.equal(sample(x, u, top_k=k), sample(x, u))
